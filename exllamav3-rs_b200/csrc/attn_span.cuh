@@ -1,0 +1,56 @@
+// What the attention over spans of the cache shares: which keys a sequence's rows see, and where they stand.
+//
+//   o[row, h] = sum_j w_j v[j] / sum_j w_j,   w_j = exp(scale * q[row, h] . k[j, h / G]),   j over the keys that the row sees
+//   window: j <= p and (j > p - window or j < sinks);   shared prefix: j <= p;   p = cached tokens + number of the row in its sequence
+//
+// A row whose span is empty gives zeros.  Keys of a block-table entry outside the pool are left out, and entries without a visible key are
+// not read.
+#pragma once
+#include "common.cuh"
+
+namespace exl3 {
+
+struct SpanArgs {
+    const half* q; half* o;                       // [rows, nq, 128]
+    const half* kc; const half* vc;               // [pages, 256, nkv, 128]
+    const int32_t* block_table;                   // [bsz, pps]
+    const int32_t* seqlens;                       // [bsz] cached tokens in front of a sequence's rows
+    const int32_t* cu_q;                          // [bsz + 1], or NULL: q_len rows each
+    const int32_t* group_start;                   // [n_groups + 1] first sequence of every group (shared prefixes), or NULL
+    const int32_t* prefix_lens;                   // [n_groups]
+    int bsz, q_len, rows, nq, nkv, pages, pps, n_groups;
+    int window, sinks;                            // window: INT_MAX without one
+    float scale_log2;
+};
+
+constexpr int SPAN_MAX_LEN = 1 << 30;
+
+// A sequence's place in the call.  ql 0: it has no rows, more than the call declared, or rows that the call does not have.
+struct SpanSeq { int row_base, ql, cached; };
+__device__ __forceinline__ SpanSeq span_seq(const SpanArgs& a, int b)
+{
+    SpanSeq s;
+    s.row_base = a.cu_q ? a.cu_q[b] : b * a.q_len;
+    s.ql = a.cu_q ? a.cu_q[b + 1] - s.row_base : a.q_len;
+    if (s.ql < 0 || s.ql > a.q_len || s.row_base < 0 || s.row_base > a.rows - s.ql) s.ql = 0;
+    s.cached = max(min(a.seqlens[b], SPAN_MAX_LEN), -SPAN_MAX_LEN);
+    return s;
+}
+
+// The group of a sequence: its first sequence, whose table has the prefix, and the prefix's tokens.  A sequence of no group, or one that
+// has not cached the whole prefix, has none and is computed on its own.
+struct SpanGroup { int g, first, len; };
+__device__ __forceinline__ SpanGroup span_group(const SpanArgs& a, int b, int cached)
+{
+    SpanGroup r = {-1, b, 0};
+    if (a.n_groups == 0) return r;
+    int lo = 0, hi = a.n_groups;                  // group_start[lo] <= b
+    if (a.group_start[0] > b || a.group_start[hi] <= b) return r;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.group_start[mid] <= b) lo = mid; else hi = mid; }
+    const int len = min(a.prefix_lens[lo], a.pps * EXL3_PAGE);
+    if (len <= 0 || len > cached) return r;
+    r.g = lo; r.first = max(a.group_start[lo], 0); r.len = len;
+    return r;
+}
+
+}  // namespace exl3

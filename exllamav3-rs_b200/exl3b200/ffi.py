@@ -65,6 +65,11 @@ def lib():
         L.exl3_gemm.argtypes = [C.c_void_p] * 8 + [C.c_int] * 7
         L.exl3_bighead_attn_paged.argtypes = [C.c_void_p] * 11 + [C.c_int] * 10 + [C.c_float]
         L.exl3_bighead_attn_paged_q.argtypes = [C.c_void_p] * 13 + [C.c_int] * 12 + [C.c_float] * 2
+        for n, planes, bits in (("exl3_rope_append_paged", 2, 0), ("exl3_rope_append_paged_q", 4, 2)):
+            getattr(L, n).argtypes = ([C.c_void_p] * 7 + [C.c_int, C.c_void_p, C.c_int, C.c_char_p] + [C.c_void_p] * 2 + [C.c_float] * 2 +
+                                      [C.c_int, C.c_float] + [C.c_void_p] * (planes + 3) + [C.c_int] * (8 + bits))
+        L.exl3_window_attn_paged.argtypes = [C.c_void_p] * 9 + [C.c_int] * 10 + [C.c_float]
+        L.exl3_prefix_attn_paged.argtypes = [C.c_void_p] * 10 + [C.c_int, C.c_void_p] + [C.c_int] * 8 + [C.c_float]
         L.exl3_graph_new.restype = C.c_void_p
         L.exl3_graph_new.argtypes = [C.c_void_p]
         L.exl3_side_stream.restype = C.c_void_p
@@ -420,6 +425,115 @@ class Ctx:
                                                  _adr(v_cache), _adr(block_table), _adr(cache_seqlens), _adr(cu_q),
                                                  _adr(o), bsz, q_len, kv_append, nq, nkv, hd, k_cache.shape[0], pps,
                                                  kv_chunk_size, int(causal), sm_scale), "bighead_attn_paged")
+
+    @staticmethod
+    def _packed(q, cu_q, max_q_len, bsz, what):
+        """(rows, row bound, heads) of q [bsz,q_len,heads,128], or [rows,heads,128] with cu_q"""
+        shape = q.shape
+        if len(shape) != (4 if cu_q is None else 3) or (cu_q is None and shape[0] != bsz) or (cu_q is not None and cu_q.numel() != bsz + 1):
+            raise Exl3Error(f"{what}: shape mismatch")
+        if cu_q is None:
+            return bsz * shape[1], shape[1], shape[2]
+        return shape[0], shape[0] if max_q_len is None else max_q_len, shape[1]
+
+    def _on_device(self, q, what):
+        if q.get_device() != self.device:
+            raise Exl3Error(f"{what}: tensors must be on the context's device")
+
+    def _rope_append(self, q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, what):
+        f16 = torch.float16
+        _chk(q, f16, "q"); _chk(k, f16, "k"); _chk(v, f16, "v"); _chk(out_q, f16, "out_q"); _chk(q_norm, f16, "q_norm"); _chk(k_norm, f16, "k_norm")
+        _chk(inv_freq, torch.float32, "inv_freq"); _chk(block_table, torch.int32, "block_table"); _chk(cache_seqlens, torch.int32, "cache_seqlens")
+        _chk(cu_q, torch.int32, "cu_q"); _chk(positions, torch.int32, "positions")
+        self._on_device(k, what)
+        bsz, pps = block_table.shape
+        rows, seq, nkv = self._packed(k, cu_q, max_q_len, bsz, what)
+        n_freq = 0 if inv_freq is None else inv_freq.numel()
+        n_axes = 1
+        if positions is not None:
+            n_axes = positions.shape[0] if positions.dim() == 2 else 1
+            if positions.numel() != n_axes * rows:
+                raise Exl3Error(f"{what}: positions must be [rows] or [axes, rows]")
+        hd = k.shape[-1]
+        if (v.shape != k.shape or cache_seqlens.numel() != bsz or (q is not None and (q.shape[:-2] != k.shape[:-2] or q.shape[-1] != hd)) or
+                (out_q is not None and (q is None or out_q.shape != q.shape)) or (freq_axis is not None and len(freq_axis) != n_freq) or
+                (q_norm is not None and q_norm.numel() != hd) or (k_norm is not None and k_norm.numel() != hd)):
+            raise Exl3Error(f"{what}: shape mismatch")
+        return bsz, pps, rows, seq, 0 if q is None else q.shape[-2], nkv, hd, n_freq, n_axes, None if freq_axis is None else bytes(freq_axis)
+
+    def rope_append_paged(self, q, k, v, k_cache, v_cache, block_table, cache_seqlens, inv_freq, out_q=None, cu_q=None, max_q_len=None,
+                          positions=None, freq_axis=None, q_norm=None, k_norm=None, norm_eps=1e-6, norm_constant_bias=0.0,
+                          rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
+        """Head norm and rotation of q and k, k and v into the fp16 pools, one launch.  positions: None, int32 [rows] or
+        [axes, rows]; freq_axis: the axis of every frequency (bytes, or a list of them).  out_q None: q in place."""
+        (bsz, pps, rows, seq, nq, nkv, hd, n_freq, n_axes, axis) = self._rope_append(
+            q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, "rope_append_paged")
+        _chk(k_cache, torch.float16, "k_cache"); _chk(v_cache, torch.float16, "v_cache")
+        if k_cache.shape[1:] != (256, nkv, hd) or v_cache.shape != k_cache.shape:
+            raise Exl3Error("rope_append_paged: the pools must be [pages, 256, nkv, head_dim]")
+        rc = lib().exl3_rope_append_paged(self._h, self._stream(stream), _adr(q), _adr(out_q), k.data_ptr(), v.data_ptr(), _adr(inv_freq),
+                                          n_freq, _adr(positions), n_axes, axis, _adr(q_norm), _adr(k_norm), norm_eps, norm_constant_bias,
+                                          rope_mode, attn_factor, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                                          cache_seqlens.data_ptr(), _adr(cu_q), bsz, seq, rows, nq, nkv, hd, k_cache.shape[0], pps)
+        if rc:
+            self.check(rc, "rope_append_paged")
+
+    def rope_append_paged_q(self, q, k, v, qk, sk, qv, sv, block_table, cache_seqlens, inv_freq, out_q=None, cu_q=None, max_q_len=None,
+                            positions=None, freq_axis=None, q_norm=None, k_norm=None, norm_eps=1e-6, norm_constant_bias=0.0,
+                            rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
+        """The same into the quantised pools (qk/qv int32 [pages,256,groups*bits], sk/sv fp16 [pages,256,groups])."""
+        (bsz, pps, rows, seq, nq, nkv, hd, n_freq, n_axes, axis) = self._rope_append(
+            q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, "rope_append_paged_q")
+        _chk(qk, torch.int32, "qk"); _chk(qv, torch.int32, "qv"); _chk(sk, torch.float16, "sk"); _chk(sv, torch.float16, "sv")
+        groups = nkv * hd // 32
+        if (sk.shape[1:] != (256, groups) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
+                qk.shape[2] % groups or qv.shape[2] % groups):
+            raise Exl3Error("rope_append_paged_q: the pools do not have the heads of k")
+        rc = lib().exl3_rope_append_paged_q(self._h, self._stream(stream), _adr(q), _adr(out_q), k.data_ptr(), v.data_ptr(), _adr(inv_freq),
+                                            n_freq, _adr(positions), n_axes, axis, _adr(q_norm), _adr(k_norm), norm_eps, norm_constant_bias,
+                                            rope_mode, attn_factor, qk.data_ptr(), sk.data_ptr(), qv.data_ptr(), sv.data_ptr(),
+                                            block_table.data_ptr(), cache_seqlens.data_ptr(), _adr(cu_q), bsz, seq, rows, nq, nkv, hd,
+                                            sk.shape[0], pps, qk.shape[2] // groups, qv.shape[2] // groups)
+        if rc:
+            self.check(rc, "rope_append_paged_q")
+
+    def _span_shapes(self, q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, what):
+        f16, i32 = torch.float16, torch.int32
+        _chk(q, f16, "q"); _chk(k_cache, f16, "k_cache"); _chk(v_cache, f16, "v_cache"); _chk(o, f16, "o")
+        _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens"); _chk(cu_q, i32, "cu_q")
+        self._on_device(q, what)
+        bsz, pps = block_table.shape
+        rows, q_len, nq = self._packed(q, cu_q, max_q_len, bsz, what)
+        pages, page, nkv, hd = k_cache.shape
+        if page != 256 or v_cache.shape != k_cache.shape or o.shape != q.shape or q.shape[-1] != hd or cache_seqlens.numel() != bsz:
+            raise Exl3Error(f"{what}: shape mismatch")
+        return bsz, q_len, rows, nq, nkv, hd, pages, pps
+
+    def window_attn_paged(self, q, k_cache, v_cache, block_table, cache_seqlens, o, window, sinks=0, sm_scale=0.0, cu_q=None,
+                          max_q_len=None, stream=None):
+        """Attention of q over the fp16 pools, each row seeing its last `window` tokens (itself among them) and the first
+        `sinks` of its sequence; the rows' own keys are in the pools already."""
+        shape = self._span_shapes(q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, "window_attn_paged")
+        rc = lib().exl3_window_attn_paged(self._h, self._stream(stream), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                          block_table.data_ptr(), cache_seqlens.data_ptr(), _adr(cu_q), o.data_ptr(), *shape, window, sinks,
+                                          sm_scale)
+        if rc:
+            self.check(rc, "window_attn_paged")
+
+    def prefix_attn_paged(self, q, k_cache, v_cache, block_table, cache_seqlens, group_start, prefix_lens, o, sm_scale=0.0, cu_q=None,
+                          max_q_len=None, stream=None):
+        """Causal attention of q over the fp16 pools; sequences [group_start[g], group_start[g+1]) share their first
+        prefix_lens[g] tokens, which are read once.  The rows' own keys are in the pools already."""
+        shape = self._span_shapes(q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, "prefix_attn_paged")
+        _chk(group_start, torch.int32, "group_start"); _chk(prefix_lens, torch.int32, "prefix_lens")
+        n_groups = prefix_lens.numel()
+        if group_start.numel() != n_groups + 1:
+            raise Exl3Error("prefix_attn_paged: group_start must have one entry more than prefix_lens")
+        rc = lib().exl3_prefix_attn_paged(self._h, self._stream(stream), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                          block_table.data_ptr(), cache_seqlens.data_ptr(), _adr(cu_q), group_start.data_ptr(),
+                                          prefix_lens.data_ptr(), n_groups, o.data_ptr(), *shape, sm_scale)
+        if rc:
+            self.check(rc, "prefix_attn_paged")
 
     def bighead_attn(self, q, k, v, o, causal=True, sm_scale=0.0, kv_chunk_size=256, stream=None):
         """src/ffi.rs:458-460: attention over plain tensors q, o [bsz,q_len,nq,hd], k, v [bsz,kv_len,nkv,hd]."""

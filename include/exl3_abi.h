@@ -196,6 +196,56 @@ EXL3_API int exl3_bighead_attn_paged_q(exl3_ctx* ctx, exl3_stream stream, const 
                               int pages, int pages_per_seq, int k_bits, int v_bits, int kv_chunk_size, int causal,
                               float sm_scale, float compand_a);
 
+/* No counterpart in the reference.  The three operators of an attention layer whose cache is not simply read whole; all over fp16 pools
+ * [pages,256,nkv,128], with the block tables, lengths and ragged form of exl3_bighead_attn_paged: q, o, k, v [bsz,q_len,heads,128], or
+ * with cu_q (int32 [bsz+1], device) packed [rows,heads,128], sequence b owning rows [cu_q[b], cu_q[b+1]); `rows` is the number of
+ * packed rows (bsz * q_len without cu_q), `q_len` (`seq`) an upper bound on the rows of one sequence.  Row i of sequence b stands at
+ * position cache_seqlens[b] + i.  Rows that belong to no sequence, and those of a sequence with more rows than declared, are left as they
+ * are.  The context's device must be the current one.  A call under stream capture keeps its pointers and sizes; lengths, tables and
+ * groups are read by the kernels at every replay.
+ *
+ * Rotation and append in one launch: out_q = R(N(q)) (out_q NULL: in place), k_cache[slot] = R(N(k)), v_cache[slot] = v.
+ * N: x * rsqrt(mean(x^2) + norm_eps) * (w + norm_constant_bias) with fp16 weights q_norm / k_norm [128], or nothing where NULL.
+ * R: rope_mode as in exl3_rope over the first 2 * n_freq dims (NEOX: n_freq % 8 == 0) by angles inv_freq[f] * position, times
+ * attn_factor; the angle is formed in 64 bits and everything else in 32, rounded once to fp16 (exl3_rope, which follows the reference,
+ * rounds between norm and rotation and forms the angle in 32 bits).  Positions: NULL = the row's position; else int32
+ * [n_axes, rows] on the device, frequency f turning by positions[freq_axis[f], row] (time, height and width of an image token).
+ * freq_axis is a HOST array of n_freq bytes, copied by the call (NULL: all 0).  Keys go to the row's position in its block table, whatever
+ * `positions` says; a row whose position is behind the table, or on an entry outside the pool, is rotated and not appended.
+ * nq may be 0 with q NULL.  q, out_q, k, v must not overlap the pools. */
+EXL3_API int exl3_rope_append_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, void* out_q, const void* k, const void* v,
+                           const float* inv_freq, int n_freq, const int32_t* positions, int n_axes, const uint8_t* freq_axis,
+                           const void* q_norm, const void* k_norm, float norm_eps, float norm_constant_bias, int rope_mode,
+                           float attn_factor, void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* cache_seqlens,
+                           const int32_t* cu_q, int bsz, int seq, int rows, int nq, int nkv, int hd, int pages, int pages_per_seq);
+/* The same into quantised pools (exl3_bighead_attn_paged_q), codes of the keys and values rounded to fp16 as exl3_quant_cache_paged makes
+ * them. */
+EXL3_API int exl3_rope_append_paged_q(exl3_ctx* ctx, exl3_stream stream, const void* q, void* out_q, const void* k, const void* v,
+                             const float* inv_freq, int n_freq, const int32_t* positions, int n_axes, const uint8_t* freq_axis,
+                             const void* q_norm, const void* k_norm, float norm_eps, float norm_constant_bias, int rope_mode,
+                             float attn_factor, void* qk, void* sk, void* qv, void* sv, const int32_t* block_table,
+                             const int32_t* cache_seqlens, const int32_t* cu_q, int bsz, int seq, int rows, int nq, int nkv, int hd,
+                             int pages, int pages_per_seq, int k_bits, int v_bits);
+
+/* Attention with a sliding window and first tokens that stay visible: the row at position p sees keys j <= p with j > p - window or
+ * j < sinks (window >= 1, sinks >= 0).  The call's own keys are in the pools already (exl3_rope_append_paged,
+ * exl3_paged_kv_cache_update).  Block-table entries none of whose keys is visible are not read, so pages behind the window can be
+ * released (and their entries be -1); the keys of an entry outside the pool are left out.  A row that sees nothing gives zeros.  sm_scale
+ * 0 = 1/sqrt(hd), negative ones are refused. */
+EXL3_API int exl3_window_attn_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, const void* k_cache, const void* v_cache,
+                           const int32_t* block_table, const int32_t* cache_seqlens, const int32_t* cu_q, void* o, int bsz, int q_len,
+                           int rows, int nq, int nkv, int hd, int pages, int pages_per_seq, int window, int sinks, float sm_scale);
+
+/* Causal attention (keys j <= p) of a batch whose sequences share prefixes: group g is the sequences [group_start[g], group_start[g+1])
+ * (int32 [n_groups+1], device, ascending), whose first prefix_lens[g] tokens (int32 [n_groups], device) are the same - the same pages,
+ * as exl3_pool_alloc_prefix gives them, or copies - and are read once for the whole group, through the block table of its first sequence.
+ * The keys behind them, and all keys of sequences in no group, are read through a sequence's own table.  A sequence that has cached less
+ * than the prefix is computed on its own.  Otherwise as above. */
+EXL3_API int exl3_prefix_attn_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, const void* k_cache, const void* v_cache,
+                           const int32_t* block_table, const int32_t* cache_seqlens, const int32_t* cu_q, const int32_t* group_start,
+                           const int32_t* prefix_lens, int n_groups, void* o, int bsz, int q_len, int rows, int nq, int nkv, int hd,
+                           int pages, int pages_per_seq, float sm_scale);
+
 /* exl3_shim_quant_cache_paged (src/ffi.rs:141-146, csrc/exl3_shim.cpp:231-240 -> kernels/cache/q_cache.cu:146-258).
  * k_in,v_in [bsz,seq,nkv*hd] fp16 contiguous (in_contiguous must be 1) -> codes/scales at cache_seqlens[b]+s.
  * page_size must be 256; bits 2..8; compand_a must be 0.  cu_q: ragged form as above. */
