@@ -2,13 +2,14 @@
 #include <limits.h>
 #include <math.h>
 #include "attn_span.cuh"
+#include "attn_rows.cuh"
 
 namespace {
 
 using namespace exl3;
 
-// The plain kernel: a warp per (row, head), one key at a time, lane = 4 dims.
-__global__ void __launch_bounds__(256) span_plain_kernel(const SpanArgs a, int early)
+// The plain kernel: a warp per (row, head), one key at a time, lane = 4 dims.  Sequences with more than `few` (query, head) rows per kv head.
+__global__ void __launch_bounds__(256) span_plain_kernel(const SpanArgs a, int few, int early)
 {
     pdl_enter_first(early);
     const int lane = threadIdx.x & 31;
@@ -22,7 +23,7 @@ __global__ void __launch_bounds__(256) span_plain_kernel(const SpanArgs a, int e
         b = lo;
     } else b = row / a.q_len;
     const SpanSeq s = span_seq(a, b);
-    if (row < s.row_base || row >= s.row_base + s.ql) return;
+    if (row < s.row_base || row >= s.row_base + s.ql || s.ql * (a.nq / a.nkv) <= few) return;
     const int p = s.cached + (row - s.row_base), end = min(p + 1, a.pps * EXL3_PAGE);
     const SpanGroup g = span_group(a, b, s.cached);
     const uint2 qr = reinterpret_cast<const uint2*>(a.q + ((size_t)row * a.nq + head) * 128)[lane];
@@ -74,12 +75,91 @@ int span_check(exl3_ctx* ctx, const SpanArgs& a, int hd, float sm_scale, const c
     return EXL3_OK;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn span_encode_tiled()
+{
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)ptr;
+        else
+            cudaGetLastError();
+    }
+    return fn;
+}
+
+// A pool as {64 dims, 256 tokens, 2 halves of a head, heads, pages}: a box of `tokens` and `halves` lands as halves of 128-byte rows in the
+// 128-byte swizzle.
+bool span_map(const SpanArgs& a, const void* pool, int tokens, int halves, CUtensorMap* map)
+{
+    EncodeTiledFn enc = span_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t tok = (cuuint64_t)a.nkv * 256;
+    cuuint64_t dims[5] = {64, EXL3_PAGE, 2, (cuuint64_t)a.nkv, (cuuint64_t)a.pages};
+    cuuint64_t strides[4] = {tok, 128, 256, EXL3_PAGE * tok};
+    cuuint32_t box[5] = {64, (cuuint32_t)tokens, (cuuint32_t)halves, 1, 1};
+    cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Kern>
+bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
+{
+    if (device >= 0 && device < 64 && done[device]) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) { cudaGetLastError(); return false; }
+    if (device >= 0 && device < 64) done[device] = true;
+    return true;
+}
+
+// the sequences of few rows
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, size_t* ws_off)
+{
+    ArMaps maps;
+    if (!span_map(a, a.kc, AR_TK, 2, &maps.k) || !span_map(a, a.vc, AR_TK, 2, &maps.v) || !span_map(a, a.kc, 16, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, &maps.v16))
+        return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+    static bool done[64] = {};
+    if (!span_configure(attn_rows_kernel, ArSmem::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    const int ctas = 2 * ctx->num_sms;
+    ArParams p;
+    p.a = a; p.min_share = 2;
+    p.partial = (float*)exl3_ws_take(ctx, ws_off, (size_t)2 * ctas * AR_ROWS * AR_MS * 4);
+    if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
+    p.counters = ctx->counters; p.status = ctx->status;
+    for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
+        p.b0 = b0; p.bsz = min(AR_MAX_BSZ, a.bsz - b0);
+        p.first = first || b0 > 0;                          // launches of one call share the partial sums
+        // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
+        const long long most = min((long long)a.pps * (EXL3_PAGE / AR_TK),
+                                   ((long long)min(a.window, SPAN_MAX_LEN) + AR_ROWS) / AR_TK + 2 + min(a.sinks, SPAN_MAX_LEN) / AR_TK + 1);
+        const int grid = (int)min((long long)ctas, max(1LL, (most * p.bsz * a.nkv + p.min_share - 1) / p.min_share));
+        if (p.first) exl3_launch_first(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p);
+        else exl3_launch(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p, 0);
+        ctx->launches++;
+    }
+    return EXL3_OK;
+}
+
 int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what)
 {
     if (span_empty(a)) return EXL3_OK;
-    const long long warps = (long long)a.rows * a.nq;
-    exl3_launch_first(ctx, span_plain_kernel, (unsigned)((warps + 7) / 8), 256, 0, st, a);
-    ctx->launches++;
+    size_t off = 0;
+    const int G = a.nq / a.nkv;
+    const bool few = G <= AR_ROWS && a.n_groups == 0;
+    if (few) {
+        const int rc = span_rows(ctx, st, a, true, &off);
+        if (rc) return rc;
+    }
+    if (!few || (long long)a.q_len * G > AR_ROWS) {
+        const long long warps = (long long)a.rows * a.nq;
+        exl3_launch_first(ctx, span_plain_kernel, (unsigned)((warps + 7) / 8), 256, 0, st, a, few ? AR_ROWS : 0);
+        ctx->launches++;
+    }
     return exl3_check_launch(ctx, what);
 }
 

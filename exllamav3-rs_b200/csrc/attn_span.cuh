@@ -54,3 +54,23 @@ __device__ __forceinline__ SpanGroup span_group(const SpanArgs& a, int b, int ca
 }
 
 }  // namespace exl3
+
+namespace exl3 {
+
+// The key tiles that a run of rows at positions p_first..p_last sees: `sink` tiles from 0 on, then tiles first .. first + near - 1.  Keys in
+// front of key_lo are not part of it.
+struct SpanTiles { int sink, first, near, lo, end; };
+template <int TK>
+__device__ __forceinline__ SpanTiles span_tiles(const SpanArgs& a, int p_first, int p_last, int key_lo)
+{
+    SpanTiles t;
+    t.end = min(max(p_last + 1, 0), a.pps * EXL3_PAGE);
+    t.lo = max(key_lo, a.window > p_first ? 0 : p_first - a.window + 1);
+    t.first = t.lo / TK;
+    t.near = t.end > t.lo ? (t.end + TK - 1) / TK - t.first : 0;
+    t.sink = (min(a.sinks, t.end) + TK - 1) / TK;
+    if (t.near > 0) t.sink = min(t.sink, t.first);
+    return t;
+}
+
+}  // namespace exl3
