@@ -22,7 +22,7 @@ constexpr int AR_TK = 64, AR_ROWS = 16, AR_STAGES = 3, AR_WARPS = 4;
 constexpr int AR_THREADS = (AR_WARPS + 1) * 32;
 constexpr int AR_HALF = AR_TK * 128;                    // bytes of one 64-dim half of a tile: rows of 128 bytes, 128-byte swizzle
 constexpr int AR_STAGE = 4 * AR_HALF;                   // K and V
-constexpr int AR_MS = 132;                              // floats per row of a partial sum: 128 dims, maximum, sum
+constexpr int AR_MS = SPAN_PART;
 constexpr int AR_MAX_BSZ = 1024;                        // sequences of a launch: their tile counts are summed in shared memory
 constexpr int AR_UNITS = AR_STAGES + 1;                 // unit descriptors: the producer is at most AR_STAGES tiles, so units, ahead
 
@@ -49,6 +49,8 @@ struct ArParams {
     float* partial;                                     // [2 * CTAs][16][AR_MS]
     int* counters;                                      // [CTAs], zero between calls
     int* status;
+    const float* prefix;                                // [splits][rows][nq][AR_MS] partial sums of the groups' prefixes, by the kernel in front
+    const int* chunk;                                   // key tiles per split of it
     int first;                                          // nothing of this call is in front of the launch
 };
 
@@ -389,6 +391,7 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
             finish = s_last != 0;
             __threadfence();
         }
+        if (finish && u.group >= 0 && !waited) { asm volatile("griddepcontrol.wait;" ::: "memory"); waited = true; }
         if (finish) {
             const int n_parts = u.whole ? 1 : u.pieces;
             for (int r = warp; r < n_rows; r += AR_WARPS) {
@@ -410,9 +413,17 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
                     l += x.y * sc;
                     acc.x += v.x * sc; acc.y += v.y * sc; acc.z += v.z * sc; acc.w += v.w * sc;
                 }
-                const float inv = l > 0.f ? 1.0f / l : 0.f;
                 const int qi = r / G, head = u.kvh * G + (r - qi * G);
-                reinterpret_cast<uint2*>(a.o)[((size_t)(u.row_base + qi) * a.nq + head) * 32 + lane] =
+                const size_t at = (size_t)(u.row_base + qi) * a.nq + head;
+                if (u.group >= 0) {
+                    AsSum all = {acc, top, l};
+                    const int pre = as_splits((u.key_lo + AS_TK - 1) / AS_TK, *p.chunk);
+                    #pragma unroll 4
+                    for (int i = 0; i < pre; ++i) as_add(all, p.prefix + ((size_t)i * a.rows * a.nq + at) * AR_MS, lane);
+                    acc = all.acc; l = all.l;
+                }
+                const float inv = l > 0.f ? 1.0f / l : 0.f;
+                reinterpret_cast<uint2*>(a.o)[at * 32 + lane] =
                     make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
             }
         }

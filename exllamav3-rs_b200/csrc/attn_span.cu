@@ -1,57 +1,12 @@
 // exl3_window_attn_paged and exl3_prefix_attn_paged: attention over spans of the paged cache.
+#include <algorithm>
 #include <limits.h>
 #include <math.h>
-#include "attn_span.cuh"
-#include "attn_rows.cuh"
+#include "attn_span_tc.cuh"
 
 namespace {
 
 using namespace exl3;
-
-// The plain kernel: a warp per (row, head), one key at a time, lane = 4 dims.  Sequences with more than `few` (query, head) rows per kv head.
-__global__ void __launch_bounds__(256) span_plain_kernel(const SpanArgs a, int few, int early)
-{
-    pdl_enter_first(early);
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (w >= (long long)a.rows * a.nq) return;
-    const int row = (int)(w / a.nq), head = (int)(w % a.nq), kvh = head / (a.nq / a.nkv);
-    int b = 0;
-    if (a.cu_q) {
-        int lo = 0, hi = a.bsz;
-        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.cu_q[mid] <= row) lo = mid; else hi = mid; }
-        b = lo;
-    } else b = row / a.q_len;
-    const SpanSeq s = span_seq(a, b);
-    if (row < s.row_base || row >= s.row_base + s.ql || s.ql * (a.nq / a.nkv) <= few) return;
-    const int p = s.cached + (row - s.row_base), end = min(p + 1, a.pps * EXL3_PAGE);
-    const SpanGroup g = span_group(a, b, s.cached);
-    const uint2 qr = reinterpret_cast<const uint2*>(a.q + ((size_t)row * a.nq + head) * 128)[lane];
-    const float2 q0 = __half22float2(*reinterpret_cast<const half2*>(&qr.x)), q1 = __half22float2(*reinterpret_cast<const half2*>(&qr.y));
-    const int near = a.window > p ? 0 : p - a.window + 1;
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = a.sinks > 0 ? 0 : near; j < end; ++j) {
-        if (j < near && j >= a.sinks) j = near;
-        if (j >= end) break;
-        const int page = a.block_table[(size_t)(j < g.len ? g.first : b) * a.pps + (j >> 8)];
-        if (page < 0 || page >= a.pages) continue;
-        const size_t at = (((size_t)page * EXL3_PAGE + (j & 255)) * a.nkv + kvh) * 32 + lane;
-        const uint2 kr = reinterpret_cast<const uint2*>(a.kc)[at], vr = reinterpret_cast<const uint2*>(a.vc)[at];
-        const float2 k0 = __half22float2(*reinterpret_cast<const half2*>(&kr.x)), k1 = __half22float2(*reinterpret_cast<const half2*>(&kr.y));
-        const float2 v0 = __half22float2(*reinterpret_cast<const half2*>(&vr.x)), v1 = __half22float2(*reinterpret_cast<const half2*>(&vr.y));
-        float x = q0.x * k0.x + q0.y * k0.y + q1.x * k1.x + q1.y * k1.y;
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        x *= a.scale_log2;
-        const float mn = fmaxf(m, x), c = m == -INFINITY ? 0.f : exp2f(m - mn), e = mn == -INFINITY ? 0.f : exp2f(x - mn);
-        m = mn; l = l * c + e;
-        acc[0] = acc[0] * c + e * v0.x; acc[1] = acc[1] * c + e * v0.y; acc[2] = acc[2] * c + e * v1.x; acc[3] = acc[3] * c + e * v1.y;
-    }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const half2 o0 = __floats2half2_rn(acc[0] * inv, acc[1] * inv), o1 = __floats2half2_rn(acc[2] * inv, acc[3] * inv);
-    reinterpret_cast<uint2*>(a.o + ((size_t)row * a.nq + head) * 128)[lane] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&o0), *reinterpret_cast<const uint32_t*>(&o1));
-}
 
 // a call without rows touches none of its tensors, whose pointers may be null then
 bool span_empty(const SpanArgs& a) { return a.bsz == 0 || a.q_len == 0 || a.rows == 0; }
@@ -118,7 +73,7 @@ bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
 }
 
 // the sequences of few rows
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, size_t* ws_off)
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsParams* prefix, size_t* ws_off)
 {
     ArMaps maps;
     if (!span_map(a, a.kc, AR_TK, 2, &maps.k) || !span_map(a, a.vc, AR_TK, 2, &maps.v) || !span_map(a, a.kc, 16, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, &maps.v16))
@@ -131,13 +86,14 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, siz
     p.partial = (float*)exl3_ws_take(ctx, ws_off, (size_t)2 * ctas * AR_ROWS * AR_MS * 4);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
+    p.prefix = prefix ? prefix->partial : nullptr; p.chunk = prefix ? prefix->chunk : nullptr;
     for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
-        p.b0 = b0; p.bsz = min(AR_MAX_BSZ, a.bsz - b0);
+        p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
         // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
-        const long long most = min((long long)a.pps * (EXL3_PAGE / AR_TK),
-                                   ((long long)min(a.window, SPAN_MAX_LEN) + AR_ROWS) / AR_TK + 2 + min(a.sinks, SPAN_MAX_LEN) / AR_TK + 1);
-        const int grid = (int)min((long long)ctas, max(1LL, (most * p.bsz * a.nkv + p.min_share - 1) / p.min_share));
+        const long long most = std::min((long long)a.pps * (EXL3_PAGE / AR_TK),
+                                        ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / AR_TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / AR_TK + 1);
+        const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * a.nkv + p.min_share - 1) / p.min_share));
         if (p.first) exl3_launch_first(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p);
         else exl3_launch(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p, 0);
         ctx->launches++;
@@ -150,14 +106,46 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     if (span_empty(a)) return EXL3_OK;
     size_t off = 0;
     const int G = a.nq / a.nkv;
-    const bool few = G <= AR_ROWS && a.n_groups == 0;
-    if (few) {
-        const int rc = span_rows(ctx, st, a, true, &off);
+    const long long packed = (long long)a.q_len * G;
+    const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long), tc = any_long || a.n_groups > 0;
+    AsParams p;
+    p.a = a;
+    int join = 0;
+    if (tc) {
+        // row blocks: at most one more per sequence (and group) than their rows fill
+        const long long filled = (long long)a.rows * G / AS_ROWS;
+        const long long own = any_long ? std::min((long long)a.bsz * ((packed + AS_ROWS - 1) / AS_ROWS), filled + a.bsz) : 0;
+        const long long units = (own + (a.n_groups ? filled + a.n_groups : 0)) * a.nkv;
+        p.slots = 2 * ctx->num_sms; p.n_seqs = any_long ? a.bsz : 0; p.status = ctx->status;
+        p.max_items = (int)std::max((long long)p.slots, units * (units < 2 * p.slots ? 2 : 1));
+        // splits: as many as a quarter of the scratch holds partial sums for, twice where prefixes have their own
+        const size_t per = (size_t)a.rows * a.nq * SPAN_PART * 4 * (a.n_groups ? 2 : 1);
+        p.max_splits = (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / per));
+        p.own_base = a.n_groups ? p.max_splits : 0;
+        join = any_long && (p.max_splits > 1 || a.n_groups > 0);
+        p.chunk = (int*)exl3_ws_take(ctx, &off, sizeof(int));
+        p.partial = join || a.n_groups ? (float*)exl3_ws_take(ctx, &off, per * p.max_splits) : nullptr;
+        if (!p.chunk || ((join || a.n_groups) && !p.partial)) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
+        CUtensorMap kmap, vmap;
+        if (!span_map(a, a.kc, AS_TK, 2, &kmap) || !span_map(a, a.vc, AS_TK, 2, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+        static bool done[64] = {};
+        if (!span_configure(attn_span_kernel, AS_SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+        if (any_few) {                                       // nothing is launched where the other kernel would be refused
+            size_t probe = off;
+            if (!exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4))
+                return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
+        }
+        exl3_launch_first(ctx, attn_span_kernel, p.max_items, AS_THREADS, AS_SMEM, st, kmap, vmap, p);
+        ctx->launches++;
+    }
+    exl3_chain_scope chain(ctx, tc);
+    if (any_few) {
+        const int rc = span_rows(ctx, st, a, !tc, tc && a.n_groups ? &p : nullptr, &off);
         if (rc) return rc;
     }
-    if (!few || (long long)a.q_len * G > AR_ROWS) {
-        const long long warps = (long long)a.rows * a.nq;
-        exl3_launch_first(ctx, span_plain_kernel, (unsigned)((warps + 7) / 8), 256, 0, st, a, few ? AR_ROWS : 0);
+    if (join) {
+        exl3_chain_scope behind(ctx);
+        exl3_launch(ctx, attn_span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 7) / 8), 256, 0, st, p);
         ctx->launches++;
     }
     return exl3_check_launch(ctx, what);

@@ -73,4 +73,22 @@ __device__ __forceinline__ SpanTiles span_tiles(const SpanArgs& a, int p_first, 
     return t;
 }
 
+// Partial sums of a row and head: 128 dims, the exponents' reference, the sum of the weights
+constexpr int SPAN_PART = 132;
+constexpr int AS_TK = 128;                               // key tile of the tcgen05 kernel, in which splits of a prefix are counted
+__device__ __forceinline__ int as_splits(int tiles, int chunk) { return max(1, (tiles + chunk - 1) / chunk); }
+
+// A row's sum, to which one part after the other is added.  Lane = four dims; all lanes have top and l.
+struct AsSum { float4 acc; float top, l; };
+__device__ __forceinline__ void as_add(AsSum& s, const float* part, int lane)
+{
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + lane);
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(part + 128));
+    const float top = fmaxf(s.top, x.x);
+    const float c0 = s.top == -INFINITY ? 0.f : exp2f(s.top - top), c1 = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+    s.acc.x = s.acc.x * c0 + v.x * c1; s.acc.y = s.acc.y * c0 + v.y * c1; s.acc.z = s.acc.z * c0 + v.z * c1; s.acc.w = s.acc.w * c0 + v.w * c1;
+    s.l = s.l * c0 + x.y * c1;
+    s.top = top;
+}
+
 }  // namespace exl3

@@ -16,12 +16,11 @@
 // to the softmax warpgroups (setmaxnreg), which need over 200 to keep 64 scores and their exponentials in flight.
 // Every mbarrier wait is bounded; a wait that runs out sets the status word and the CTA leaves through the tear-down.
 #pragma once
-#include "attn_paged.cuh"
-#include "gemm_tc.cuh"
+#include "attn_tc_ops.cuh"
 
 namespace exl3 {
 
-constexpr int ATC_ROWS = 128, ATC_NB = 2, ATC_CTA_ROWS = ATC_ROWS * ATC_NB, ATC_TN = 128, ATC_D = 128;
+constexpr int ATC_ROWS = 128, ATC_NB = 2, ATC_CTA_ROWS = ATC_ROWS * ATC_NB;
 constexpr int ATC_KV_SLOTS = 5;                               // ring of K / V tile buffers
 constexpr int ATC_THREADS = ATC_NB * 128 + 128;                // two softmax warpgroups + one service warpgroup
 constexpr int ATC_Q_BYTES = ATC_ROWS * ATC_D * 2;             // per block, 32 KB: two 64-wide d blocks of 16 KB
@@ -32,79 +31,6 @@ constexpr int ATC_OFF_BAR = ATC_OFF_KV + ATC_KV_SLOTS * ATC_KV_SLOT;
 // q_full[NB], kv_full/kv_empty[slots], s_full[NB], p_full[NB], o_full
 constexpr int ATC_NBARS = ATC_NB + 2 * ATC_KV_SLOTS + 2 * ATC_NB + 1;
 constexpr int ATC_SMEM = ATC_OFF_BAR + ATC_NBARS * 8 + 16 + 1024;
-constexpr float ATC_RESCALE_THRESHOLD = 8.0f;                 // log2 units
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar)
-{
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tc_st32(uint32_t taddr, const float (&v)[32])
-{
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
-}
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// MN-major (N contiguous), 128-byte swizzled B tile: 64-element N atoms `lbo` bytes apart, 8-row K groups 1024 bytes apart
-__device__ __forceinline__ uint64_t tc_smem_desc_mn(const void* p, uint32_t lbo)
-{
-    const uint32_t a = smem_u32(p);
-    uint64_t d = 0;
-    d |= (uint64_t)((a >> 4) & 0x3fff);
-    d |= (uint64_t)((lbo >> 4) & 0x3fff) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
-constexpr uint32_t ATC_IDESC_S  = (1u << 4) | ((uint32_t)(ATC_TN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);            // N = 128 keys
-constexpr uint32_t ATC_IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(ATC_D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); // B MN-major, N = 128
-
-
-
-// D[tmem] (+)= A[tmem, packed fp16] * B[smem desc]
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
-{
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void tc_st32u(uint32_t taddr, const uint32_t (&r)[32])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
-}
-
-__device__ __forceinline__ void tc_st16u(uint32_t taddr, const uint32_t (&r)[16])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ float ex2_approx(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// two exponentials per special-function operation: 2^x of an fp16 pair (the result is used as fp16 anyway)
-__device__ __forceinline__ uint32_t ex2_h2(uint32_t x)
-{
-    uint32_t y;
-    asm("ex2.approx.f16x2 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
 #ifndef ATC_EXP_F16X2
 #define ATC_EXP_F16X2 0
 #endif
@@ -113,14 +39,6 @@ __device__ __forceinline__ uint32_t ex2_h2(uint32_t x)
 // three - needs about 230 registers; at 184 it spills and ran at 278 us against 162 us on 4 x 256 query rows.)
 #define ATC_REG_SOFTMAX 184
 #define ATC_REG_SERVICE 120
-__device__ __forceinline__ float fmax3(float a, float b, float c)
-{
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
-
 // grid (max_items, nkv); kmap / vmap: 4-D maps of the pools {D, nkv, 256, pages}, box {64, 1, 128, 1}, 128B swizzle.
 // The plan's chunk must be a multiple of 128 keys.
 __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
