@@ -73,7 +73,7 @@ bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
 }
 
 // the sequences of few rows
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsParams* prefix, size_t* ws_off)
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsJoin& join, size_t* ws_off)
 {
     ArMaps maps;
     if (!span_map(a, a.kc, AR_TK, 2, &maps.k) || !span_map(a, a.vc, AR_TK, 2, &maps.v) || !span_map(a, a.kc, 16, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, &maps.v16))
@@ -86,7 +86,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
     p.partial = (float*)exl3_ws_take(ctx, ws_off, (size_t)2 * ctas * AR_ROWS * AR_MS * 4);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
-    p.prefix = prefix ? prefix->partial : nullptr; p.chunk = prefix ? prefix->chunk : nullptr;
+    p.prefix = join.prefix; p.chunk = join.prefix_chunk;
     for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
         p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
@@ -101,51 +101,73 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
     return EXL3_OK;
 }
 
+// a launch of the tcgen05 kernel with NB row blocks per CTA
+template <int NB>
+int span_tc(exl3_ctx* ctx, cudaStream_t st, AsParams& p, long long units)
+{
+    CUtensorMap kmap, vmap;
+    if (!span_map(p.a, p.a.kc, AS_TK, 2, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+    static bool done[64] = {};
+    if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    p.slots = AsCfg<NB>::CTAS * ctx->num_sms;
+    p.max_items = (int)std::max((long long)p.slots, units * (units < 2 * p.slots ? 2 : 1));
+    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, p.max_items, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p);
+    else exl3_launch(ctx, attn_span_kernel<NB>, p.max_items, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p, 0);
+    ctx->launches++;
+    return EXL3_OK;
+}
+
 int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what)
 {
     if (span_empty(a)) return EXL3_OK;
-    size_t off = 0;
     const int G = a.nq / a.nkv;
-    const long long packed = (long long)a.q_len * G;
-    const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long), tc = any_long || a.n_groups > 0;
-    AsParams p;
-    p.a = a;
-    int join = 0;
-    if (tc) {
-        // row blocks: at most one more per sequence (and group) than their rows fill
-        const long long filled = (long long)a.rows * G / AS_ROWS;
-        const long long own = any_long ? std::min((long long)a.bsz * ((packed + AS_ROWS - 1) / AS_ROWS), filled + a.bsz) : 0;
-        const long long units = (own + (a.n_groups ? filled + a.n_groups : 0)) * a.nkv;
-        p.slots = 2 * ctx->num_sms; p.n_seqs = any_long ? a.bsz : 0; p.status = ctx->status;
-        p.max_items = (int)std::max((long long)p.slots, units * (units < 2 * p.slots ? 2 : 1));
-        // splits: as many as a quarter of the scratch holds partial sums for, twice where prefixes have their own
-        const size_t per = (size_t)a.rows * a.nq * SPAN_PART * 4 * (a.n_groups ? 2 : 1);
-        p.max_splits = (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / per));
-        p.own_base = a.n_groups ? p.max_splits : 0;
-        join = any_long && (p.max_splits > 1 || a.n_groups > 0);
-        p.chunk = (int*)exl3_ws_take(ctx, &off, sizeof(int));
-        p.partial = join || a.n_groups ? (float*)exl3_ws_take(ctx, &off, per * p.max_splits) : nullptr;
-        if (!p.chunk || ((join || a.n_groups) && !p.partial)) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
-        CUtensorMap kmap, vmap;
-        if (!span_map(a, a.kc, AS_TK, 2, &kmap) || !span_map(a, a.vc, AS_TK, 2, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
-        static bool done[64] = {};
-        if (!span_configure(attn_span_kernel, AS_SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
-        if (any_few) {                                       // nothing is launched where the other kernel would be refused
-            size_t probe = off;
-            if (!exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4))
-                return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
-        }
-        exl3_launch_first(ctx, attn_span_kernel, p.max_items, AS_THREADS, AS_SMEM, st, kmap, vmap, p);
-        ctx->launches++;
+    const long long packed = (long long)a.q_len * G, all = (long long)a.rows * G;
+    const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long), groups = a.n_groups > 0;
+    // Splits: as many as a quarter of the scratch holds partial sums for.  Prefixes always leave some, a sequence's own span where it is
+    // split or a prefix is added to it.
+    const size_t per = (size_t)a.rows * a.nq * SPAN_PART * 4 * (groups && any_long ? 2 : 1);
+    const int splits = (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / per));
+    const bool join = any_long && (splits > 1 || groups);
+    size_t off = 0;
+    AsJoin j = {a, nullptr, nullptr, nullptr, nullptr, AS_BLOCK};
+    int* chunk = (int*)exl3_ws_take(ctx, &off, 2 * sizeof(int));
+    float* part[2] = {};
+    const size_t region = (size_t)a.rows * a.nq * SPAN_PART * 4 * splits;
+    if (groups) part[0] = (float*)exl3_ws_take(ctx, &off, region);
+    if (join) part[1] = (float*)exl3_ws_take(ctx, &off, region);
+    size_t probe = off;
+    if (!chunk || (groups && !part[0]) || (join && !part[1]) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4)))
+        return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
+    AsParams p = {a, nullptr, nullptr, ctx->status, 0, splits, 0, 0, 1};
+    int rc = EXL3_OK;
+    if (groups) {
+        // two row blocks share the tiles where a group may have that many rows
+        const bool two = all > (long long)AS_BLOCK * a.n_groups;
+        p.prefixes = 1; p.partial = part[0]; p.chunk = chunk;
+        j.prefix = part[0]; j.prefix_chunk = chunk;
+        const long long units = (all / (two ? 2 * AS_BLOCK : AS_BLOCK) + a.n_groups) * a.nkv;
+        rc = two ? span_tc<2>(ctx, st, p, units) : span_tc<1>(ctx, st, p, units);
+        if (rc) return rc;
+        p.first = 0;
     }
-    exl3_chain_scope chain(ctx, tc);
+    exl3_chain_scope chain(ctx, groups);
+    if (any_long) {
+        const bool two = packed > AS_BLOCK;
+        const int rows = two ? 2 * AS_BLOCK : AS_BLOCK;
+        p.prefixes = 0; p.partial = part[1]; p.chunk = chunk + 1;
+        j.own = part[1]; j.own_chunk = chunk + 1; j.own_rows = rows;
+        const long long units = std::min((long long)a.bsz * ((packed + rows - 1) / rows), all / rows + a.bsz) * a.nkv;
+        rc = two ? span_tc<2>(ctx, st, p, units) : span_tc<1>(ctx, st, p, units);
+        if (rc) return rc;
+        p.first = 0;
+    }
+    exl3_chain_scope behind(ctx, p.first == 0);
     if (any_few) {
-        const int rc = span_rows(ctx, st, a, !tc, tc && a.n_groups ? &p : nullptr, &off);
+        rc = span_rows(ctx, st, a, p.first != 0, j, &off);
         if (rc) return rc;
     }
     if (join) {
-        exl3_chain_scope behind(ctx);
-        exl3_launch(ctx, attn_span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 7) / 8), 256, 0, st, p);
+        exl3_launch(ctx, attn_span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 7) / 8), 256, 0, st, j);
         ctx->launches++;
     }
     return exl3_check_launch(ctx, what);
