@@ -49,8 +49,7 @@ struct ArParams {
     float* partial;                                     // [2 * CTAs][16][AR_MS]
     int* counters;                                      // [CTAs], zero between calls
     int* status;
-    const float* prefix;                                // [splits][rows][nq][AR_MS] partial sums of the groups' prefixes, by the kernel in front
-    const int* chunk;                                   // key tiles per split of it
+    float* rest;                                        // [rows][nq][AR_MS] partial sums of sequences that a prefix is added to
     int first;                                          // nothing of this call is in front of the launch
 };
 
@@ -217,7 +216,7 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
         return r;
     };
     const int g = lane >> 2, t4 = lane & 3;
-    bool waited = p.first, ok = true;
+    bool ok = true;
     int it = 0, n_unit = 0;
     for (long long f = f0; f < f1 && ok; ++n_unit) {
         if (!mbar_wait_warp(&full[it % AR_STAGES], (it / AR_STAGES) & 1)) { ok = false; break; }
@@ -391,45 +390,40 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
             finish = s_last != 0;
             __threadfence();
         }
-        if (finish && u.group >= 0 && !waited) { asm volatile("griddepcontrol.wait;" ::: "memory"); waited = true; }
         if (finish) {
-            const int n_parts = u.whole ? 1 : u.pieces;
-            for (int r = warp; r < n_rows; r += AR_WARPS) {
-                auto part = [&](int i) -> const float* {
-                    return u.whole ? merge + r * AR_MS : p.partial + ((size_t)(2 * (u.c0 + i) + (i == 0 ? 1 : 0)) * AR_ROWS + r) * AR_MS;
-                };
-                float top = -INFINITY;
-                for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, u.whole ? part(i)[128] : __ldcg(part(i) + 128));
+            constexpr int U = AR_ROWS / AR_WARPS;           // a warp's rows: warp, warp + 4, ..
+            bool on[U];
+            SpanSum sum[U];
+            size_t at[U];
+            #pragma unroll
+            for (int i = 0; i < U; ++i) {
+                on[i] = warp + AR_WARPS * i < n_rows;
+                const int r = on[i] ? warp + AR_WARPS * i : 0, qi = r / G;       // (a row that is not there stands for the first one)
+                at[i] = (size_t)(u.row_base + qi) * a.nq + u.kvh * G + (r - qi * G);
+            }
+            if (u.whole) {
                 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float l = 0.f;
-                #pragma unroll 4
-                for (int i = 0; i < n_parts; ++i) {
-                    const float* s = part(i);
-                    const float4 v = u.whole ? reinterpret_cast<const float4*>(s)[lane] : __ldcg(reinterpret_cast<const float4*>(s) + lane);
-                    const float2 x = u.whole ? *reinterpret_cast<const float2*>(s + 128) : __ldcg(reinterpret_cast<const float2*>(s + 128));
-                    const float sc = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
-                    l += x.y * sc;
-                    acc.x += v.x * sc; acc.y += v.y * sc; acc.z += v.z * sc; acc.w += v.w * sc;
+                for (int i = 0; i < U; ++i) {
+                    const float* row = merge + (warp + AR_WARPS * i) * AR_MS;
+                    if (on[i]) sum[i] = {reinterpret_cast<const float4*>(row)[lane], row[128], row[129]};
                 }
-                const int qi = r / G, head = u.kvh * G + (r - qi * G);
-                const size_t at = (size_t)(u.row_base + qi) * a.nq + head;
-                if (u.group >= 0) {
-                    AsSum all = {acc, top, l};
-                    const int pre = as_splits((u.key_lo + AS_TK - 1) / AS_TK, *p.chunk);
-                    #pragma unroll 4
-                    for (int i = 0; i < pre; ++i) as_add(all, p.prefix + ((size_t)i * a.rows * a.nq + at) * AR_MS, lane);
-                    acc = all.acc; l = all.l;
+            } else
+                span_merge(sum, u.pieces, [&](int k, int i) -> const float* {
+                    return p.partial + ((size_t)(2 * (u.c0 + k) + (k == 0 ? 1 : 0)) * AR_ROWS + (on[i] ? warp + AR_WARPS * i : 0)) * AR_MS; },
+                    [](int, int) { return true; }, lane);
+            #pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (!on[i]) continue;
+                if (u.group < 0) reinterpret_cast<uint2*>(a.o)[at[i] * 32 + lane] = span_result(sum[i]);
+                else {                                          // span_join_kernel adds the prefix
+                    reinterpret_cast<float4*>(p.rest + at[i] * AR_MS)[lane] = sum[i].acc;
+                    if (lane == 0) *reinterpret_cast<float2*>(p.rest + at[i] * AR_MS + 128) = make_float2(sum[i].top, sum[i].l);
                 }
-                const float inv = l > 0.f ? 1.0f / l : 0.f;
-                reinterpret_cast<uint2*>(a.o)[at * 32 + lane] =
-                    make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
             }
         }
         if (!(ok = rendezvous())) break;                // the buffer is free again
     }
-    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!p.first) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!ok && lane == 0) atomicExch(p.status, 3);
 }
 

@@ -20,6 +20,7 @@ int span_check(exl3_ctx* ctx, const SpanArgs& a, int hd, float sm_scale, const c
         return bad(EXL3_ERR_INVALID, "bad shape");
     if (!a.cu_q && (long long)a.bsz * a.q_len != a.rows) return bad(EXL3_ERR_INVALID, "rows must be bsz * q_len without cu_q");
     if (a.nq % a.nkv != 0) return bad(EXL3_ERR_INVALID, "n_q_heads must be a multiple of n_kv_heads");
+    if (a.bsz > 32 * AS_MAX_CHUNKS) return bad(EXL3_ERR_UNSUPPORTED, "more than 8192 sequences");
     if ((long long)a.rows * a.nq > 1LL << 30) return bad(EXL3_ERR_INVALID, "too many rows");
     if (hd != 128) return bad(EXL3_ERR_UNSUPPORTED, "head_dim must be 128");
     if (!span_empty(a) && (!a.q || !a.o || !a.kc || !a.vc || !a.block_table || !a.seqlens)) return bad(EXL3_ERR_INVALID, "null argument");
@@ -73,7 +74,7 @@ bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
 }
 
 // the sequences of few rows
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsJoin& join, size_t* ws_off)
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsParams& pre, size_t* ws_off)
 {
     ArMaps maps;
     if (!span_map(a, a.kc, AR_TK, 2, &maps.k) || !span_map(a, a.vc, AR_TK, 2, &maps.v) || !span_map(a, a.kc, 16, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, &maps.v16))
@@ -86,7 +87,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
     p.partial = (float*)exl3_ws_take(ctx, ws_off, (size_t)2 * ctas * AR_ROWS * AR_MS * 4);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
-    p.prefix = join.prefix; p.chunk = join.prefix_chunk;
+    p.rest = pre.rest;
     for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
         p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
@@ -103,16 +104,15 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
 
 // a launch of the tcgen05 kernel with NB row blocks per CTA
 template <int NB>
-int span_tc(exl3_ctx* ctx, cudaStream_t st, AsParams& p, long long units)
+int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p)
 {
     CUtensorMap kmap, vmap;
     if (!span_map(p.a, p.a.kc, AS_TK, 2, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     static bool done[64] = {};
     if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
-    p.slots = AsCfg<NB>::CTAS * ctx->num_sms;
-    p.max_items = (int)std::max((long long)p.slots, units * (units < 2 * p.slots ? 2 : 1));
-    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, p.max_items, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p);
-    else exl3_launch(ctx, attn_span_kernel<NB>, p.max_items, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p, 0);
+    const int grid = AsCfg<NB>::CTAS * ctx->num_sms;
+    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p);
+    else exl3_launch(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p, 0);
     ctx->launches++;
     return EXL3_OK;
 }
@@ -123,51 +123,43 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     const int G = a.nq / a.nkv;
     const long long packed = (long long)a.q_len * G, all = (long long)a.rows * G;
     const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long), groups = a.n_groups > 0;
-    // Splits: as many as a quarter of the scratch holds partial sums for.  Prefixes always leave some, a sequence's own span where it is
-    // split or a prefix is added to it.
-    const size_t per = (size_t)a.rows * a.nq * SPAN_PART * 4 * (groups && any_long ? 2 : 1);
-    const int splits = (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / per));
-    const bool join = any_long && (splits > 1 || groups);
+    // Two row blocks share the tiles where a group or a sequence may have that many rows
+    const bool two_prefix = all > (long long)AS_BLOCK * a.n_groups, two_own = packed > AS_BLOCK;
+    // Scratch.  Prefixes: a place per row, head and part, as many parts as a quarter of the scratch has room for, and one for
+    // the sequence's rest.  Own spans: two units per CTA.
+    const size_t place = (size_t)a.rows * a.nq * SPAN_PART * 4;
+    AsParams p = {a, 0, nullptr, nullptr, (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / place)), nullptr,
+                  ctx->counters + 1024, ctx->status, 1};
     size_t off = 0;
-    AsJoin j = {a, nullptr, nullptr, nullptr, nullptr, AS_BLOCK};
-    int* chunk = (int*)exl3_ws_take(ctx, &off, 2 * sizeof(int));
-    float* part[2] = {};
-    const size_t region = (size_t)a.rows * a.nq * SPAN_PART * 4 * splits;
-    if (groups) part[0] = (float*)exl3_ws_take(ctx, &off, region);
-    if (join) part[1] = (float*)exl3_ws_take(ctx, &off, region);
+    int* share = (int*)exl3_ws_take(ctx, &off, 2 * sizeof(int));
+    float* prefix = groups ? (float*)exl3_ws_take(ctx, &off, place * p.max_splits) : nullptr;
+    if (groups) p.rest = (float*)exl3_ws_take(ctx, &off, place);
+    float* own = any_long ? (float*)exl3_ws_take(ctx, &off, (size_t)2 * ctx->num_sms * 2 * AS_BLOCK * SPAN_PART * 4) : nullptr;
     size_t probe = off;
-    if (!chunk || (groups && !part[0]) || (join && !part[1]) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4)))
+    if (!share || (groups && (!prefix || !p.rest)) || (any_long && !own) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4)))
         return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
-    AsParams p = {a, nullptr, nullptr, ctx->status, 0, splits, 0, 0, 1};
     int rc = EXL3_OK;
     if (groups) {
-        // two row blocks share the tiles where a group may have that many rows
-        const bool two = all > (long long)AS_BLOCK * a.n_groups;
-        p.prefixes = 1; p.partial = part[0]; p.chunk = chunk;
-        j.prefix = part[0]; j.prefix_chunk = chunk;
-        const long long units = (all / (two ? 2 * AS_BLOCK : AS_BLOCK) + a.n_groups) * a.nkv;
-        rc = two ? span_tc<2>(ctx, st, p, units) : span_tc<1>(ctx, st, p, units);
+        p.prefixes = 1; p.partial = prefix; p.share = share;
+        rc = two_prefix ? span_tc<2>(ctx, st, p) : span_tc<1>(ctx, st, p);
         if (rc) return rc;
         p.first = 0;
     }
     exl3_chain_scope chain(ctx, groups);
     if (any_long) {
-        const bool two = packed > AS_BLOCK;
-        const int rows = two ? 2 * AS_BLOCK : AS_BLOCK;
-        p.prefixes = 0; p.partial = part[1]; p.chunk = chunk + 1;
-        j.own = part[1]; j.own_chunk = chunk + 1; j.own_rows = rows;
-        const long long units = std::min((long long)a.bsz * ((packed + rows - 1) / rows), all / rows + a.bsz) * a.nkv;
-        rc = two ? span_tc<2>(ctx, st, p, units) : span_tc<1>(ctx, st, p, units);
+        p.prefixes = 0; p.partial = own; p.share = share + 1;
+        rc = two_own ? span_tc<2>(ctx, st, p) : span_tc<1>(ctx, st, p);
         if (rc) return rc;
         p.first = 0;
     }
-    exl3_chain_scope behind(ctx, p.first == 0);
+    exl3_chain_scope behind(ctx, any_long);
     if (any_few) {
-        rc = span_rows(ctx, st, a, p.first != 0, j, &off);
+        rc = span_rows(ctx, st, a, p.first != 0, p, &off);
         if (rc) return rc;
     }
-    if (join) {
-        exl3_launch(ctx, attn_span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 7) / 8), 256, 0, st, j);
+    if (groups) {
+        const SpanJoinParams j = {a, prefix, share, p.rest};
+        exl3_launch(ctx, span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 31) / 32), 256, 0, st, j);
         ctx->launches++;
     }
     return exl3_check_launch(ctx, what);

@@ -76,19 +76,71 @@ __device__ __forceinline__ SpanTiles span_tiles(const SpanArgs& a, int p_first, 
 // Partial sums of a row and head: 128 dims, the exponents' reference, the sum of the weights
 constexpr int SPAN_PART = 132;
 constexpr int AS_TK = 128;                               // key tile of the tcgen05 kernel, in which splits of a prefix are counted
-__device__ __forceinline__ int as_splits(int tiles, int chunk) { return max(1, (tiles + chunk - 1) / chunk); }
+// Partial sums that a unit of so many tiles can have where CTAs take `share` tiles each; 0: units are not cut
+__device__ __forceinline__ int span_places(int tiles, int share) { return share > 0 ? (tiles - 1) / share + 2 : 1; }
 
-// A row's sum, to which one part after the other is added.  Lane = four dims; all lanes have top and l.
-struct AsSum { float4 acc; float top, l; };
-__device__ __forceinline__ void as_add(AsSum& s, const float* part, int lane)
+// Sums of U rows over n parts each.  A warp; lane = four dims, all lanes have top and l.  part(k, u): part k of row u,
+// there(k, u): whether the row has it.  What waits for memory
+// is asked for together: the maxima and sums of all parts, and the values of four parts of every row, whatever the maxima are (a part
+// without keys, or a place that nobody wrote values to, has weight 0 and is not looked at).  One after the other, 4 us per row.
+struct SpanSum { float4 acc; float top, l; };
+template <int U, typename Part, typename There>
+__device__ __forceinline__ void span_merge(SpanSum (&s)[U], int n, Part part, There there, int lane)
 {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + lane);
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(part + 128));
-    const float top = fmaxf(s.top, x.x);
-    const float c0 = s.top == -INFINITY ? 0.f : exp2f(s.top - top), c1 = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
-    s.acc.x = s.acc.x * c0 + v.x * c1; s.acc.y = s.acc.y * c0 + v.y * c1; s.acc.z = s.acc.z * c0 + v.z * c1; s.acc.w = s.acc.w * c0 + v.w * c1;
-    s.l = s.l * c0 + x.y * c1;
-    s.top = top;
+    constexpr int AHEAD = 4;
+    #pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        const int cnt = min(32, n - k0);
+        float2 x[U];
+        float4 v[AHEAD][U];
+        auto fetch = [&](int k) {
+            #pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                #pragma unroll
+                for (int u = 0; u < U; ++u) v[i][u] = __ldcg(reinterpret_cast<const float4*>(part(k0 + min(k + i, cnt - 1), u)) + lane);
+        };
+        #pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = __ldcg(reinterpret_cast<const float2*>(part(k0 + min(lane, cnt - 1), u) + 128));
+        fetch(0);
+        float w[U];
+        #pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (lane >= cnt || !there(k0 + lane, u)) x[u] = make_float2(-INFINITY, 0.f);
+            float top = x[u].x;
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, s[u].top);
+            w[u] = x[u].x == -INFINITY ? 0.f : exp2f(x[u].x - top);
+            float l = x[u].y * w[u];
+            if (x[u].x == -INFINITY) l = 0.f;
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const float c = s[u].top == -INFINITY ? 0.f : exp2f(s[u].top - top);
+            s[u].acc.x *= c; s[u].acc.y *= c; s[u].acc.z *= c; s[u].acc.w *= c;
+            s[u].l = s[u].l * c + l;
+            s[u].top = top;
+        }
+        for (int k = 0; k < cnt; k += AHEAD) {
+            #pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                #pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float wk = __shfl_sync(0xffffffffu, w[u], min(k + i, 31));
+                    if (k + i < cnt && wk != 0.f) {
+                        s[u].acc.x = fmaf(v[i][u].x, wk, s[u].acc.x); s[u].acc.y = fmaf(v[i][u].y, wk, s[u].acc.y);
+                        s[u].acc.z = fmaf(v[i][u].z, wk, s[u].acc.z); s[u].acc.w = fmaf(v[i][u].w, wk, s[u].acc.w);
+                    }
+                }
+            if (k + AHEAD < cnt) fetch(k + AHEAD);
+        }
+    }
+}
+__device__ __forceinline__ uint2 span_result(const SpanSum& s)
+{
+    const float inv = s.l > 0.f ? 1.0f / s.l : 0.f;
+    const half2 a = __floats2half2_rn(s.acc.x * inv, s.acc.y * inv), b = __floats2half2_rn(s.acc.z * inv, s.acc.w * inv);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
 }  // namespace exl3
