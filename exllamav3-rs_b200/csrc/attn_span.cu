@@ -49,16 +49,16 @@ EncodeTiledFn span_encode_tiled()
     return fn;
 }
 
-// A pool as {64 dims, 256 tokens, 2 halves of a head, heads, pages}: a box of `tokens` and `halves` lands as halves of 128-byte rows in the
-// 128-byte swizzle.
-bool span_map(const SpanArgs& a, const void* pool, int tokens, int halves, CUtensorMap* map)
+// A pool as {64 dims, 256 tokens, 2 halves of a head, heads, pages}: a box lands as heads of halves of 128-byte rows, a row per token, in
+// the 128-byte swizzle.
+bool span_map(const SpanArgs& a, const void* pool, int tokens, int halves, int heads, CUtensorMap* map)
 {
     EncodeTiledFn enc = span_encode_tiled();
     if (!enc) return false;
     const cuuint64_t tok = (cuuint64_t)a.nkv * 256;
     cuuint64_t dims[5] = {64, EXL3_PAGE, 2, (cuuint64_t)a.nkv, (cuuint64_t)a.pages};
     cuuint64_t strides[4] = {tok, 128, 256, EXL3_PAGE * tok};
-    cuuint32_t box[5] = {64, (cuuint32_t)tokens, (cuuint32_t)halves, 1, 1};
+    cuuint32_t box[5] = {64, (cuuint32_t)tokens, (cuuint32_t)halves, (cuuint32_t)heads, 1};
     cuuint32_t one[5] = {1, 1, 1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -73,18 +73,27 @@ bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
     return true;
 }
 
-// the sequences of few rows
+// the sequences of few rows, HW heads side by side
+constexpr size_t AR_SCRATCH = (size_t)AR_WARPS * AR_ROWS * AR_MS * 4;       // per CTA and place, at most
+#ifndef AR_MIN_KEYS
+#define AR_MIN_KEYS 128
+#endif
+template <int HW>
 int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsParams& pre, size_t* ws_off)
 {
+    using Cfg = ArCfg<HW>;
     ArMaps maps;
-    if (!span_map(a, a.kc, AR_TK, 2, &maps.k) || !span_map(a, a.vc, AR_TK, 2, &maps.v) || !span_map(a, a.kc, 16, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, &maps.v16))
+    if (!span_map(a, a.kc, Cfg::TK, 2, HW, &maps.k) || !span_map(a, a.vc, Cfg::TK, 2, HW, &maps.v) ||
+        (Cfg::KW > 1 && (!span_map(a, a.kc, 16, 1, 1, &maps.k16) || !span_map(a, a.vc, 16, 1, 1, &maps.v16))))
         return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+    if (Cfg::KW == 1) { maps.k16 = maps.k; maps.v16 = maps.v; }
     static bool done[64] = {};
-    if (!span_configure(attn_rows_kernel, ArSmem::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    if (!span_configure(attn_rows_kernel<HW>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int ctas = 2 * ctx->num_sms;
     ArParams p;
-    p.a = a; p.min_share = 2;
-    p.partial = (float*)exl3_ws_take(ctx, ws_off, (size_t)2 * ctas * AR_ROWS * AR_MS * 4);
+    p.a = a;
+    p.min_share = AR_MIN_KEYS / Cfg::TK;
+    p.partial = (float*)exl3_ws_take(ctx, ws_off, 2 * ctas * AR_SCRATCH);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
     p.rest = pre.rest;
@@ -92,11 +101,11 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
         p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
         // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
-        const long long most = std::min((long long)a.pps * (EXL3_PAGE / AR_TK),
-                                        ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / AR_TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / AR_TK + 1);
-        const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * a.nkv + p.min_share - 1) / p.min_share));
-        if (p.first) exl3_launch_first(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p);
-        else exl3_launch(ctx, attn_rows_kernel, grid, AR_THREADS, ArSmem::BYTES, st, maps, p, 0);
+        const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
+                                        ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1);
+        const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
+        if (p.first) exl3_launch_first(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
+        else exl3_launch(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
         ctx->launches++;
     }
     return EXL3_OK;
@@ -107,7 +116,7 @@ template <int NB>
 int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p)
 {
     CUtensorMap kmap, vmap;
-    if (!span_map(p.a, p.a.kc, AS_TK, 2, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+    if (!span_map(p.a, p.a.kc, AS_TK, 2, 1, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, 1, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     static bool done[64] = {};
     if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int grid = AsCfg<NB>::CTAS * ctx->num_sms;
@@ -129,14 +138,14 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     // the sequence's rest.  Own spans: two units per CTA.
     const size_t place = (size_t)a.rows * a.nq * SPAN_PART * 4;
     AsParams p = {a, 0, nullptr, nullptr, (int)std::max((size_t)1, std::min((size_t)AS_MAX_SPLITS, ctx->ws_bytes / 4 / place)), nullptr,
-                  ctx->counters + 1024, ctx->status, 1};
+                  ctx->counters + 4096, ctx->status, 1};
     size_t off = 0;
     int* share = (int*)exl3_ws_take(ctx, &off, 2 * sizeof(int));
     float* prefix = groups ? (float*)exl3_ws_take(ctx, &off, place * p.max_splits) : nullptr;
     if (groups) p.rest = (float*)exl3_ws_take(ctx, &off, place);
     float* own = any_long ? (float*)exl3_ws_take(ctx, &off, (size_t)2 * ctx->num_sms * 2 * AS_BLOCK * SPAN_PART * 4) : nullptr;
     size_t probe = off;
-    if (!share || (groups && (!prefix || !p.rest)) || (any_long && !own) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_ROWS * AR_MS * 4)))
+    if (!share || (groups && (!prefix || !p.rest)) || (any_long && !own) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_SCRATCH)))
         return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     int rc = EXL3_OK;
     if (groups) {
@@ -154,7 +163,7 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     }
     exl3_chain_scope behind(ctx, any_long);
     if (any_few) {
-        rc = span_rows(ctx, st, a, p.first != 0, p, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, p, &off) : span_rows<1>(ctx, st, a, p.first != 0, p, &off);
         if (rc) return rc;
     }
     if (groups) {

@@ -143,4 +143,12 @@ __device__ __forceinline__ uint2 span_result(const SpanSum& s)
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+// A (row, head)'s finished sum: to the output, or to where span_join_kernel adds the prefix.  A warp, lane = four dims.
+__device__ __forceinline__ void span_put(const SpanArgs& a, float* rest, int group, size_t at, const SpanSum& s, int lane)
+{
+    if (group < 0) { reinterpret_cast<uint2*>(a.o)[at * 32 + lane] = span_result(s); return; }
+    reinterpret_cast<float4*>(rest + at * SPAN_PART)[lane] = s.acc;
+    if (lane == 0) *reinterpret_cast<float2*>(rest + at * SPAN_PART + 128) = make_float2(s.top, s.l);
+}
+
 }  // namespace exl3
