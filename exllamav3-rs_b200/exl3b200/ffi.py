@@ -5,6 +5,7 @@ library is missing or a call returns an error code, an exception is raised.
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -65,9 +66,7 @@ def lib():
         L.exl3_gemm.argtypes = [C.c_void_p] * 8 + [C.c_int] * 7
         L.exl3_bighead_attn_paged.argtypes = [C.c_void_p] * 11 + [C.c_int] * 10 + [C.c_float]
         L.exl3_bighead_attn_paged_q.argtypes = [C.c_void_p] * 13 + [C.c_int] * 12 + [C.c_float] * 2
-        for n, planes, bits in (("exl3_rope_append_paged", 2, 0), ("exl3_rope_append_paged_q", 4, 2)):
-            getattr(L, n).argtypes = ([C.c_void_p] * 7 + [C.c_int, C.c_void_p, C.c_int, C.c_char_p] + [C.c_void_p] * 2 + [C.c_float] * 2 +
-                                      [C.c_int, C.c_float] + [C.c_void_p] * (planes + 3) + [C.c_int] * (8 + bits))
+        L.exl3_rope_append_paged.argtypes = [C.c_void_p, C.c_void_p, C.c_char_p]
         L.exl3_window_attn_paged.argtypes = [C.c_void_p] * 9 + [C.c_int] * 10 + [C.c_float]
         L.exl3_prefix_attn_paged.argtypes = [C.c_void_p] * 10 + [C.c_int, C.c_void_p] + [C.c_int] * 8 + [C.c_float]
         L.exl3_graph_new.restype = C.c_void_p
@@ -87,6 +86,14 @@ def _ptr(t):
 def _adr(t):
     """address for a function whose argument types are declared"""
     return None if t is None else t.data_ptr()
+
+
+def _num(t):
+    """address for a packed structure"""
+    return 0 if t is None else t.data_ptr()
+
+
+_ROPE_APPEND = struct.Struct("@15Q3f13i64s")      # exl3_rope_append_args (include/exl3_abi.h)
 
 
 def _raw_stream():
@@ -427,86 +434,95 @@ class Ctx:
                                                  kv_chunk_size, int(causal), sm_scale), "bighead_attn_paged")
 
     @staticmethod
-    def _packed(q, cu_q, max_q_len, bsz, what):
-        """(rows, row bound, heads) of q [bsz,q_len,heads,128], or [rows,heads,128] with cu_q"""
-        shape = q.shape
-        if len(shape) != (4 if cu_q is None else 3) or (cu_q is None and shape[0] != bsz) or (cu_q is not None and cu_q.numel() != bsz + 1):
-            raise Exl3Error(f"{what}: shape mismatch")
+    def _packed(shape, cu_q, max_q_len, bsz, what):
+        """(rows, row bound, heads) of a tensor [bsz,q_len,heads,128], or [rows,heads,128] with cu_q"""
         if cu_q is None:
-            return bsz * shape[1], shape[1], shape[2]
-        return shape[0], shape[0] if max_q_len is None else max_q_len, shape[1]
+            if len(shape) == 4 and shape[0] == bsz:
+                return bsz * shape[1], shape[1], shape[2]
+        elif len(shape) == 3 and cu_q.numel() == bsz + 1:
+            return shape[0], shape[0] if max_q_len is None else max_q_len, shape[1]
+        raise Exl3Error(f"{what}: shape mismatch")
 
-    def _on_device(self, q, what):
-        if q.get_device() != self.device:
-            raise Exl3Error(f"{what}: tensors must be on the context's device")
-
-    def _rope_append(self, q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, what):
-        f16 = torch.float16
-        _chk(q, f16, "q"); _chk(k, f16, "k"); _chk(v, f16, "v"); _chk(out_q, f16, "out_q"); _chk(q_norm, f16, "q_norm"); _chk(k_norm, f16, "k_norm")
-        _chk(inv_freq, torch.float32, "inv_freq"); _chk(block_table, torch.int32, "block_table"); _chk(cache_seqlens, torch.int32, "cache_seqlens")
-        _chk(cu_q, torch.int32, "cu_q"); _chk(positions, torch.int32, "positions")
-        self._on_device(k, what)
-        bsz, pps = block_table.shape
-        rows, seq, nkv = self._packed(k, cu_q, max_q_len, bsz, what)
-        n_freq = 0 if inv_freq is None else inv_freq.numel()
+    def _rope_append(self, q, k, v, planes, bits, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm,
+                     k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream, what):
+        f16, i32 = torch.float16, torch.int32
+        _chk(k, f16, "k"); _chk(v, f16, "v"); _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens")
+        shape, table, n_freq, nq = k.shape, block_table.shape, 0, 0
+        bsz, hd = table[0], shape[-1]
+        rows, seq, nkv = self._packed(shape, cu_q, max_q_len, bsz, what)
+        pages, page = planes[0].shape[:2]
+        good = v.shape == shape and cache_seqlens.numel() == bsz and page == 256 and k.get_device() == self.device
         n_axes = 1
+        if q is not None:
+            _chk(q, f16, "q")
+            full = q.shape
+            nq = full[-2]
+            good = good and full[:-2] == shape[:-2] and full[-1] == hd
+            if out_q is not None:
+                _chk(out_q, f16, "out_q")
+                good = good and out_q.shape == full
+        if inv_freq is not None:
+            _chk(inv_freq, torch.float32, "inv_freq")
+            n_freq = inv_freq.numel()
+        if cu_q is not None:
+            _chk(cu_q, i32, "cu_q")
         if positions is not None:
-            n_axes = positions.shape[0] if positions.dim() == 2 else 1
-            if positions.numel() != n_axes * rows:
-                raise Exl3Error(f"{what}: positions must be [rows] or [axes, rows]")
-        hd = k.shape[-1]
-        if (v.shape != k.shape or cache_seqlens.numel() != bsz or (q is not None and (q.shape[:-2] != k.shape[:-2] or q.shape[-1] != hd)) or
-                (out_q is not None and (q is None or out_q.shape != q.shape)) or (freq_axis is not None and len(freq_axis) != n_freq) or
-                (q_norm is not None and q_norm.numel() != hd) or (k_norm is not None and k_norm.numel() != hd)):
-            raise Exl3Error(f"{what}: shape mismatch")
-        return bsz, pps, rows, seq, 0 if q is None else q.shape[-2], nkv, hd, n_freq, n_axes, None if freq_axis is None else bytes(freq_axis)
+            _chk(positions, i32, "positions")
+            if positions.dim() == 2:
+                n_axes = positions.shape[0]
+            good = good and positions.numel() == n_axes * rows
+        if freq_axis is not None:
+            good = good and len(freq_axis) == n_freq
+            freq_axis = bytes(freq_axis)
+        for w in (q_norm, k_norm):
+            if w is not None:
+                _chk(w, f16, "q_norm / k_norm")
+                good = good and w.numel() == hd
+        if not good or (out_q is not None and q is None) or n_freq > 64:
+            raise Exl3Error(f"{what}: shape mismatch, or tensors that are not on the context's device")
+        args = _ROPE_APPEND.pack(_num(q), _num(out_q), k.data_ptr(), v.data_ptr(), _num(inv_freq), _num(positions), _num(q_norm), _num(k_norm),
+                                 planes[0].data_ptr(), planes[1].data_ptr(), _num(planes[2]), _num(planes[3]), block_table.data_ptr(),
+                                 cache_seqlens.data_ptr(), _num(cu_q), norm_eps, norm_constant_bias, attn_factor, n_freq, n_axes, rope_mode, bsz,
+                                 seq, rows, nq, nkv, hd, pages, table[1], bits[0], bits[1], freq_axis or b"")
+        rc = lib().exl3_rope_append_paged(self._h, self._stream(stream), args)
+        if rc:
+            self.check(rc, what)
 
     def rope_append_paged(self, q, k, v, k_cache, v_cache, block_table, cache_seqlens, inv_freq, out_q=None, cu_q=None, max_q_len=None,
                           positions=None, freq_axis=None, q_norm=None, k_norm=None, norm_eps=1e-6, norm_constant_bias=0.0,
                           rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
         """Head norm and rotation of q and k, k and v into the fp16 pools, one launch.  positions: None, int32 [rows] or
         [axes, rows]; freq_axis: the axis of every frequency (bytes, or a list of them).  out_q None: q in place."""
-        (bsz, pps, rows, seq, nq, nkv, hd, n_freq, n_axes, axis) = self._rope_append(
-            q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, "rope_append_paged")
         _chk(k_cache, torch.float16, "k_cache"); _chk(v_cache, torch.float16, "v_cache")
-        if k_cache.shape[1:] != (256, nkv, hd) or v_cache.shape != k_cache.shape:
+        shape = k_cache.shape
+        if shape[2:] != k.shape[-2:] or v_cache.shape != shape:
             raise Exl3Error("rope_append_paged: the pools must be [pages, 256, nkv, head_dim]")
-        rc = lib().exl3_rope_append_paged(self._h, self._stream(stream), _adr(q), _adr(out_q), k.data_ptr(), v.data_ptr(), _adr(inv_freq),
-                                          n_freq, _adr(positions), n_axes, axis, _adr(q_norm), _adr(k_norm), norm_eps, norm_constant_bias,
-                                          rope_mode, attn_factor, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                                          cache_seqlens.data_ptr(), _adr(cu_q), bsz, seq, rows, nq, nkv, hd, k_cache.shape[0], pps)
-        if rc:
-            self.check(rc, "rope_append_paged")
+        self._rope_append(q, k, v, (k_cache, v_cache, None, None), (0, 0), block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions,
+                          freq_axis, q_norm, k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream, "rope_append_paged")
 
     def rope_append_paged_q(self, q, k, v, qk, sk, qv, sv, block_table, cache_seqlens, inv_freq, out_q=None, cu_q=None, max_q_len=None,
                             positions=None, freq_axis=None, q_norm=None, k_norm=None, norm_eps=1e-6, norm_constant_bias=0.0,
                             rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
         """The same into the quantised pools (qk/qv int32 [pages,256,groups*bits], sk/sv fp16 [pages,256,groups])."""
-        (bsz, pps, rows, seq, nq, nkv, hd, n_freq, n_axes, axis) = self._rope_append(
-            q, k, v, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, "rope_append_paged_q")
         _chk(qk, torch.int32, "qk"); _chk(qv, torch.int32, "qv"); _chk(sk, torch.float16, "sk"); _chk(sv, torch.float16, "sv")
-        groups = nkv * hd // 32
-        if (sk.shape[1:] != (256, groups) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
-                qk.shape[2] % groups or qv.shape[2] % groups):
+        groups = k.shape[-2] * k.shape[-1] // 32
+        if (sk.shape[2:] != (groups,) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
+                qk.shape[2] % groups or qv.shape[2] % groups or not qk.shape[2] or not qv.shape[2]):
             raise Exl3Error("rope_append_paged_q: the pools do not have the heads of k")
-        rc = lib().exl3_rope_append_paged_q(self._h, self._stream(stream), _adr(q), _adr(out_q), k.data_ptr(), v.data_ptr(), _adr(inv_freq),
-                                            n_freq, _adr(positions), n_axes, axis, _adr(q_norm), _adr(k_norm), norm_eps, norm_constant_bias,
-                                            rope_mode, attn_factor, qk.data_ptr(), sk.data_ptr(), qv.data_ptr(), sv.data_ptr(),
-                                            block_table.data_ptr(), cache_seqlens.data_ptr(), _adr(cu_q), bsz, seq, rows, nq, nkv, hd,
-                                            sk.shape[0], pps, qk.shape[2] // groups, qv.shape[2] // groups)
-        if rc:
-            self.check(rc, "rope_append_paged_q")
+        self._rope_append(q, k, v, (qk, qv, sk, sv), (qk.shape[2] // groups, qv.shape[2] // groups), block_table, cache_seqlens, inv_freq, out_q,
+                          cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream,
+                          "rope_append_paged_q")
 
     def _span_shapes(self, q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, what):
         f16, i32 = torch.float16, torch.int32
         _chk(q, f16, "q"); _chk(k_cache, f16, "k_cache"); _chk(v_cache, f16, "v_cache"); _chk(o, f16, "o")
         _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens"); _chk(cu_q, i32, "cu_q")
-        self._on_device(q, what)
         bsz, pps = block_table.shape
-        rows, q_len, nq = self._packed(q, cu_q, max_q_len, bsz, what)
-        pages, page, nkv, hd = k_cache.shape
-        if page != 256 or v_cache.shape != k_cache.shape or o.shape != q.shape or q.shape[-1] != hd or cache_seqlens.numel() != bsz:
-            raise Exl3Error(f"{what}: shape mismatch")
+        shape, cache = q.shape, k_cache.shape
+        rows, q_len, nq = self._packed(shape, cu_q, max_q_len, bsz, what)
+        pages, page, nkv, hd = cache
+        if page != 256 or v_cache.shape != cache or o.shape != shape or shape[-1] != hd or cache_seqlens.numel() != bsz or q.get_device() != self.device:
+            raise Exl3Error(f"{what}: shape mismatch, or tensors that are not on the context's device")
         return bsz, q_len, rows, nq, nkv, hd, pages, pps
 
     def window_attn_paged(self, q, k_cache, v_cache, block_table, cache_seqlens, o, window, sinks=0, sm_scale=0.0, cu_q=None,

@@ -206,26 +206,27 @@ EXL3_API int exl3_bighead_attn_paged_q(exl3_ctx* ctx, exl3_stream stream, const 
  *
  * Rotation and append in one launch: out_q = R(N(q)) (out_q NULL: in place), k_cache[slot] = R(N(k)), v_cache[slot] = v.
  * N: x * rsqrt(mean(x^2) + norm_eps) * (w + norm_constant_bias) with fp16 weights q_norm / k_norm [128], or nothing where NULL.
- * R: rope_mode as in exl3_rope over the first 2 * n_freq dims (NEOX: n_freq % 8 == 0) by angles inv_freq[f] * position, times
- * attn_factor; the angle is formed in 64 bits and everything else in 32, rounded once to fp16 (exl3_rope, which follows the reference,
- * rounds between norm and rotation and forms the angle in 32 bits).  Positions: NULL = the row's position; else int32
- * [n_axes, rows] on the device, frequency f turning by positions[freq_axis[f], row] (time, height and width of an image token).
- * freq_axis is a HOST array of n_freq bytes, copied by the call (NULL: all 0).  Keys go to the row's position in its block table, whatever
- * `positions` says; a row whose position is behind the table, or on an entry outside the pool, is rotated and not appended.
- * nq may be 0 with q NULL.  q, out_q, k, v must not overlap the pools. */
-EXL3_API int exl3_rope_append_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, void* out_q, const void* k, const void* v,
-                           const float* inv_freq, int n_freq, const int32_t* positions, int n_axes, const uint8_t* freq_axis,
-                           const void* q_norm, const void* k_norm, float norm_eps, float norm_constant_bias, int rope_mode,
-                           float attn_factor, void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* cache_seqlens,
-                           const int32_t* cu_q, int bsz, int seq, int rows, int nq, int nkv, int hd, int pages, int pages_per_seq);
-/* The same into quantised pools (exl3_bighead_attn_paged_q), codes of the keys and values rounded to fp16 as exl3_quant_cache_paged makes
- * them. */
-EXL3_API int exl3_rope_append_paged_q(exl3_ctx* ctx, exl3_stream stream, const void* q, void* out_q, const void* k, const void* v,
-                             const float* inv_freq, int n_freq, const int32_t* positions, int n_axes, const uint8_t* freq_axis,
-                             const void* q_norm, const void* k_norm, float norm_eps, float norm_constant_bias, int rope_mode,
-                             float attn_factor, void* qk, void* sk, void* qv, void* sv, const int32_t* block_table,
-                             const int32_t* cache_seqlens, const int32_t* cu_q, int bsz, int seq, int rows, int nq, int nkv, int hd,
-                             int pages, int pages_per_seq, int k_bits, int v_bits);
+ * R: rope_mode as in exl3_rope over the first 2 * n_freq dims (n_freq <= 64; NEOX: n_freq % 8 == 0) by angles inv_freq[f] * position,
+ * times attn_factor; the angle is formed in 64 bits and everything else in 32, rounded once to fp16 (exl3_rope, which follows the
+ * reference, rounds between norm and rotation and forms the angle in 32 bits).  Positions: NULL = the row's position; else int32
+ * [n_axes, rows] on the device, frequency f turning by positions[freq_axis[f], row] (time, height and width of an image token).  Keys
+ * go to the row's position in its block table, whatever `positions` says; a row whose position is behind the table, or on an entry
+ * outside the pool, is rotated and not appended.  nq may be 0 with q NULL.  q, out_q, k and v must not overlap the pools, and out_q not
+ * overlap q but for being it.
+ * k_bits = v_bits = 0: fp16 pools.  2..8: quantised pools (exl3_bighead_attn_paged_q), codes and scales of the keys and values rounded to
+ * fp16 as exl3_quant_cache_paged makes them. */
+typedef struct {
+    const void* q; void* out_q; const void* k; const void* v;
+    const float* inv_freq; const int32_t* positions;
+    const void* q_norm; const void* k_norm;
+    void* k_cache; void* v_cache;           /* fp16 pools, or code planes */
+    void* k_scales; void* v_scales;         /* of code planes */
+    const int32_t* block_table; const int32_t* cache_seqlens; const int32_t* cu_q;
+    float norm_eps, norm_constant_bias, attn_factor;
+    int n_freq, n_axes, rope_mode, bsz, seq, rows, nq, nkv, hd, pages, pages_per_seq, k_bits, v_bits;
+    uint8_t freq_axis[64];                  /* axis of every frequency */
+} exl3_rope_append_args;
+EXL3_API int exl3_rope_append_paged(exl3_ctx* ctx, exl3_stream stream, const exl3_rope_append_args* args);
 
 /* Attention with a sliding window and first tokens that stay visible: the row at position p sees keys j <= p with j > p - window or
  * j < sinks (window >= 1, sinks >= 0).  The call's own keys are in the pools already (exl3_rope_append_paged,

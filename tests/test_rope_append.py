@@ -259,35 +259,33 @@ def test_a_layer_of_a_decode_loop(ctx):
 
 # ------------------------------------------------------------------------------------------------------------------- refusals
 
-GOOD = dict(q=4096, out_q=0, k=4096, v=4096, inv=4096, n_freq=64, pos=0, axes=1, fa=None, qn=0, kn=0, eps=1e-6, cb=0.0, mode=2, af=1.0, kc=4096, vc=4096,
-            sk=4096, sv=4096, bt=4096, sl=4096, cu=0, bsz=2, seq=1, rows=2, nq=16, nkv=8, hd=128, pages=4, pps=2, kb=4, vb=4)
+GOOD = dict(q=4096, out_q=0, k=4096, v=4096, inv=4096, pos=0, qn=0, kn=0, kc=4096, vc=4096, sk=0, sv=0, bt=4096, sl=4096, cu=0, eps=1e-6, cb=0.0,
+            af=1.0, n_freq=64, axes=1, mode=2, bsz=2, seq=1, rows=2, nq=16, nkv=8, hd=128, pages=4, pps=2, kb=0, vb=0, fa=b"")
 BAD = [(dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(inv=0), -1), (dict(kc=0), -1), (dict(vc=0), -1), (dict(bt=0), -1), (dict(sl=0), -1),
        (dict(q=4100), -1), (dict(out_q=4100), -1), (dict(k=4104), -1), (dict(v=4104), -1), (dict(kc=4104), -1), (dict(vc=4104), -1), (dict(qn=4098), -1),
        (dict(kn=4098), -1), (dict(n_freq=0), -1), (dict(n_freq=65), -1), (dict(n_freq=12), -2), (dict(mode=7), -1), (dict(hd=64), -2), (dict(bsz=-1), -1),
        (dict(seq=-1), -1), (dict(rows=3), -1), (dict(rows=-1), -1), (dict(nq=-1), -1), (dict(nkv=0), -1), (dict(pages=0), -1), (dict(pps=0), -1),
-       (dict(axes=3), -1), (dict(pos=4096, axes=0), -1), (dict(pos=4096, axes=300), -1), (dict(pos=4096, axes=3), -1),
-       (dict(pos=4096, axes=3, fa=bytes([0, 1, 3] * 22)[:64]), -1), (dict(fa=bytes([1] * 64)), -1)]
+       (dict(axes=3), -1), (dict(pos=4096, axes=0), -1), (dict(pos=4096, axes=3, fa=bytes([0, 1, 3] * 22)[:64]), -1), (dict(fa=bytes([1] * 64)), -1),
+       (dict(kb=4, vb=4), -1)]
+QUANT = dict(kb=4, vb=8, sk=4096, sv=4096)
+BAD_QUANT = [(dict(sk=0), -1), (dict(sv=0), -1), (dict(sk=4100), -1), (dict(kb=1), -1), (dict(vb=9), -1), (dict(kb=0), -1), (dict(kc=4104), -1)]
 
 
-def _call(lib, quant, ctx, **change):
-    a = {**GOOD, **change}
-    g = lambda *names: [a[x] for x in names]  # noqa: E731
-    head = [ctx, None] + g("q", "out_q", "k", "v", "inv", "n_freq", "pos", "axes", "fa", "qn", "kn", "eps", "cb", "mode", "af")
-    tail = g("bt", "sl", "cu", "bsz", "seq", "rows", "nq", "nkv", "hd", "pages", "pps")
-    if quant:
-        return lib.exl3_rope_append_paged_q(*head, *g("kc", "sk", "vc", "sv"), *tail, a["kb"], a["vb"])
-    return lib.exl3_rope_append_paged(*head, *g("kc", "vc"), *tail)
+def _call(lib, ctx, **change):
+    import exl3b200.ffi as ffi
+    return lib.exl3_rope_append_paged(ctx, None, ffi._ROPE_APPEND.pack(*{**GOOD, **change}.values()))
 
 
-@pytest.mark.parametrize("quant", [False, True])
-def test_refusals_on_the_host(quant):
+def test_refusals_on_the_host():
     lib = _lib()
-    assert _call(lib, quant, None) == -1
+    assert _call(lib, None) == -1
     fake = C.create_string_buffer(1 << 16)
     C.memset(fake, 0xff, 4)                                # a device that never is the current one
-    for change, code in BAD + ([(dict(sk=0), -1), (dict(sv=0), -1), (dict(sk=4100), -1), (dict(kb=1), -1), (dict(vb=9), -1)] if quant else []):
-        assert _call(lib, quant, fake, **change) == code, change
-    assert _call(lib, quant, fake) == -1 and b"device" in lib.exl3_last_error(fake)
+    assert lib.exl3_rope_append_paged(fake, None, None) == -1
+    for change, code in BAD + [({**QUANT, **x}, code) for x, code in BAD_QUANT]:
+        assert _call(lib, fake, **change) == code, change
+    for change in ({}, QUANT):
+        assert _call(lib, fake, **change) == -1 and b"device" in lib.exl3_last_error(fake)
 
 
 @pytest.mark.gpu
@@ -301,6 +299,6 @@ def test_wrapper_checks_shapes(ctx):
     ctx.rope_append_paged(**good)
     for change in (dict(q=f(2, 2, 16, HD)), dict(v=f(2, 1, 4, HD)), dict(k=f(2, 8, HD)), dict(k_cache=f(2, PAGE, 4, HD)), dict(v_cache=f(3, PAGE, 8, HD)),
                    dict(cache_seqlens=i(3)), dict(positions=i(3, 3)), dict(positions=i(3, 2), freq_axis=bytes(3)), dict(out_q=f(2, 1, 8, HD)),
-                   dict(q_norm=f(64)), dict(inv_freq=f(64)), dict(positions=i(3, 2)), dict(freq_axis=[1] * 64)):
+                   dict(q_norm=f(64)), dict(inv_freq=f(64)), dict(freq_axis=[1] * 64)):
         with pytest.raises(exl3b200.Exl3Error):
             ctx.rope_append_paged(**{**good, **change})

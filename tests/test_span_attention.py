@@ -393,7 +393,8 @@ GOOD = dict(q=4096, k=4096, v=4096, bt=4096, sl=4096, cu=0, o=4096, bsz=2, q_len
 BAD = [(dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(bt=0), -1), (dict(sl=0), -1), (dict(o=0), -1), (dict(q=4098), -1), (dict(o=4104), -1),
        (dict(k=4100), -1), (dict(v=4100), -1), (dict(bsz=-1), -1), (dict(q_len=-1), -1), (dict(rows=3), -1), (dict(rows=-1), -1), (dict(nq=0), -1),
        (dict(nkv=0), -1), (dict(nq=12), -1), (dict(hd=64), -2), (dict(pages=0), -1), (dict(pps=0), -1), (dict(pps=1 << 23), -1), (dict(scale=-1.0), -1),
-       (dict(scale=math.nan), -1), (dict(scale=math.inf), -1), (dict(bsz=1 << 30, rows=1 << 30), -1)]
+       (dict(scale=math.nan), -1), (dict(scale=math.inf), -1), (dict(bsz=1 << 30, rows=1 << 30), -2), (dict(bsz=8193, rows=8193), -2),
+       (dict(nq=1 << 20, rows=1 << 11, cu=4096), -1)]
 BAD_WINDOW = [(dict(window=0), -1), (dict(window=-3), -1), (dict(sinks=-1), -1)]
 BAD_PREFIX = [(dict(groups=-1), -1), (dict(groups=3), -1), (dict(gs=0), -1), (dict(pl=0), -1)]
 
