@@ -3,8 +3,8 @@
 //
 // Bound by HBM: every visible key and value is read once, and the two products are far below what mma.sync gives.  So the work is a
 // stream: all sequences' key tiles, head group after head group, stand in one line, and every CTA takes an equal part of it, whatever the
-// lengths (148 SMs x 2 CTAs; the parts are found from the lengths by each CTA itself, so there is no list to build in front).  A
-// producer warp runs ahead through a ring of three tiles and over the borders of sequences, so that the end of one costs no loads.
+// lengths (a CTA per SM; the parts are found from the lengths by each CTA itself, so there is no list to build in front).  A
+// producer warp runs ahead through a ring of six tiles and over the borders of sequences, so that the end of one costs no loads.
 //
 // A tile is 32 KB of keys and values, for four warps: HW = 4 heads side by side and 16 keys, a head per warp, where the kv heads come in
 // fours - 1 KB of every token in one piece, and no warp needs another - else one head and 64 keys, 16 per warp, which meet at the end of
@@ -16,12 +16,12 @@
 #pragma once
 #include <cuda.h>
 #include "attn_span.cuh"
-#include "attn_paged.cuh"
+#include "attn_tc_ops.cuh"
 #include "async_copy.cuh"
 
 namespace exl3 {
 
-constexpr int AR_ROWS = 16, AR_STAGES = 3, AR_WARPS = 4;
+constexpr int AR_ROWS = 16, AR_STAGES = 6, AR_WARPS = 4;
 constexpr int AR_THREADS = (AR_WARPS + 1) * 32;
 constexpr int AR_STAGE = 32768;                         // keys and values of a tile
 constexpr int AR_MS = SPAN_PART;
@@ -42,9 +42,8 @@ struct ArCfg {
     // full[stages], empty[stages], meet; then the tile of every stage
     static constexpr int OFF_TILE = OFF_BAR + (2 * AR_STAGES + 1) * 8;
     static constexpr int BYTES = OFF_TILE + AR_STAGES * 4 + 16 + 1024;
-    static_assert(HW == 1 || HW == 4, "two heads' buffers of the merge leave no room for two CTAs per SM");
     static_assert(HW * HEAD * 2 == AR_STAGE, "a tile");
-    static_assert(2 * (BYTES + 1024 + 64) <= EXL3_SM_SMEM, "two CTAs per SM");
+    static_assert(BYTES + 1024 + 64 <= EXL3_SM_SMEM, "a CTA per SM");
     static_assert(OFF_ML % 8 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
@@ -68,7 +67,7 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 }
 
 template <int HW>
-__global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_constant__ ArMaps maps, const ArParams p, int early)
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_constant__ ArMaps maps, const ArParams p, int early)
 {
     using Cfg = ArCfg<HW>;
     constexpr int KW = Cfg::KW, TK = Cfg::TK, PER_PAGE = EXL3_PAGE / TK;
@@ -257,41 +256,59 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
         #pragma unroll
         for (int i = 0; i < 16; ++i) { o_acc[i][0] = o_acc[i][1] = o_acc[i][2] = o_acc[i][3] = 0.f; }
         float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-        for (int i = 0; i < u.tiles; ++i, ++it) {
-            const int stage = it % AR_STAGES;
-            if (i > 0 && !mbar_wait_warp(&full[stage], (it / AR_STAGES) & 1)) { ok = false; break; }
-            const int kt = tile_of[stage];
-            const int kb = kt * TK + wk * 16;                                        // first key of this warp's
-            if (kt >= 0 && kb < any_hi && (kb + 16 > any_lo || kb < a.sinks)) {
-                const uint8_t* ks_ = smem + stage * AR_STAGE + wh * Cfg::HEAD;
-                const uint8_t* vs_ = ks_ + AR_STAGE / 2;
-                float s[2][4];
+        // two tiles at a time where there are two: most of a step is latency, of which they have one
+        for (int i = 0; i < u.tiles; i += 2) {
+            const bool two = i + 1 < u.tiles;
+            const int st0 = it % AR_STAGES, st1 = two ? (it + 1) % AR_STAGES : st0;
+            if (i > 0 && !mbar_wait_warp(&full[st0], (it / AR_STAGES) & 1)) { ok = false; break; }
+            if (two && !mbar_wait_warp(&full[st1], ((it + 1) / AR_STAGES) & 1)) { ok = false; break; }
+            const int kt0 = tile_of[st0], kt1 = two ? tile_of[st1] : -1;
+            const int kb0 = kt0 * TK + wk * 16, kb1 = kt1 * TK + wk * 16;            // first key of this warp's in either
+            auto seen = [&](int kt, int kb) { return kt >= 0 && kb < any_hi && (kb + 16 > any_lo || kb < a.sinks); };
+            auto whole = [&](int kt, int kb) { return kt >= 0 && kb + 16 <= all_hi && (kb >= all_lo || kb + 16 <= a.sinks); };
+            const bool in0 = seen(kt0, kb0), in1 = seen(kt1, kb1);
+            if (in0 || in1) {
+                const uint8_t* base[2] = {smem + st0 * AR_STAGE + wh * Cfg::HEAD, smem + st1 * AR_STAGE + wh * Cfg::HEAD};
+                float s[4][4];                                                      // blocks of 8 keys, two of either tile
                 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb) {
-                    s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-                    const int r = wk * 16 + nb * 8 + (lane & 7);
-                    const uint8_t* krow = ks_ + r * 128;
+                for (int nb = 0; nb < 4; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+                #pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t kf[4][4];
                     #pragma unroll
-                    for (int ks = 0; ks < 8; ks += 2) {
-                        const int ch = ks * 2 + (lane >> 3);                         // 16-byte chunk of the row's 16
-                        uint32_t b0, b1, b2, b3;
-                        ldsm_x4(b0, b1, b2, b3, krow + (ch >> 3) * Cfg::HALF + (((ch & 7) ^ (r & 7)) << 4));
-                        mma_f16(s[nb], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], b0, b1);
-                        mma_f16(s[nb], qf[ks + 1][0], qf[ks + 1][1], qf[ks + 1][2], qf[ks + 1][3], b2, b3);
+                    for (int nb = 0; nb < 4; ++nb) {
+                        const int r = wk * 16 + (nb & 1) * 8 + (lane & 7), ch = x * 4 + (lane >> 3);      // row, 16-byte chunk of its 16
+                        ldsm_x4(kf[nb][0], kf[nb][1], kf[nb][2], kf[nb][3], base[nb >> 1] + r * 128 + (ch >> 3) * Cfg::HALF + (((ch & 7) ^ (r & 7)) << 4));
                     }
+                    #pragma unroll
+                    for (int nb = 0; nb < 4; ++nb) mma_f16(s[nb], qf[2 * x][0], qf[2 * x][1], qf[2 * x][2], qf[2 * x][3], kf[nb][0], kf[nb][1]);
+                    #pragma unroll
+                    for (int nb = 0; nb < 4; ++nb) mma_f16(s[nb], qf[2 * x + 1][0], qf[2 * x + 1][1], qf[2 * x + 1][2], qf[2 * x + 1][3], kf[nb][2], kf[nb][3]);
                 }
-                const bool clear = kb + 16 <= all_hi && (kb >= all_lo || kb + 16 <= a.sinks);      // every row sees every key
-                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};                       // values of keys that exist for some row: pairs 2 t4, + 1 and 8 on
+                // values of the first tile are asked for under the softmax, of the second under the first product
+                const int vr = wk * 16 + (lane & 15);
+                uint32_t vf[8][4];
+                auto values = [&](int tile) {
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int ch = 2 * x + (lane >> 4);
+                        ldsm_x4_t(vf[x][0], vf[x][1], vf[x][2], vf[x][3], base[tile] + AR_STAGE / 2 + vr * 128 + (ch >> 3) * Cfg::HALF + (((ch & 7) ^ (vr & 7)) << 4));
+                    }
+                };
+                values(0);
+                const bool clear = whole(kt0, kb0) && whole(kt1, kb1);              // every row sees every key of both
+                uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};      // values of keys that some row sees: pairs 2 t4, + 1 and 8 on
                 float mx[2] = {-INFINITY, -INFINITY};
                 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int nb = 0; nb < 4; ++nb)
                     #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float v = s[nb][e] * a.scale_log2;
                         if (!clear) {
-                            const int key = kb + nb * 8 + 2 * t4 + (e & 1), h = e >> 1;
-                            if (!(key < hi[h] && (key >= lo[h] || key < a.sinks))) v = -INFINITY;
-                            if (!(key < any_hi && (key >= any_lo || key < a.sinks))) keep[nb] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                            const int key = (nb < 2 ? kb0 : kb1) + (nb & 1) * 8 + 2 * t4 + (e & 1), h = e >> 1;
+                            const bool in = nb < 2 ? in0 : in1;
+                            if (!(in && key < hi[h] && (key >= lo[h] || key < a.sinks))) v = -INFINITY;
+                            if (!(in && key < any_hi && (key >= any_lo || key < a.sinks))) keep[nb] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
                         }
                         s[nb][e] = v;
                         mx[e >> 1] = fmaxf(mx[e >> 1], v);
@@ -302,7 +319,7 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                     const float m_new = fmaxf(m_run[h], mx[h]);
-                    corr[h] = m_new == -INFINITY ? 1.0f : exp2f(m_run[h] - m_new);
+                    corr[h] = m_new == -INFINITY ? 1.0f : ex2_approx(m_run[h] - m_new);
                     m_run[h] = m_new;
                     l_run[h] *= corr[h];
                     ref[h] = m_new == -INFINITY ? 0.f : m_new;       // a row that has seen nothing: exp2(-inf - 0) = 0
@@ -311,28 +328,28 @@ __global__ void __launch_bounds__(AR_THREADS, 2) attn_rows_kernel(const __grid_c
                     #pragma unroll
                     for (int d = 0; d < 16; ++d) { o_acc[d][0] *= corr[0]; o_acc[d][1] *= corr[0]; o_acc[d][2] *= corr[1]; o_acc[d][3] *= corr[1]; }
                 }
-                uint32_t pf[2][2];
+                uint32_t pf[4][2];
                 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb) {
-                    const float e0 = exp2f(s[nb][0] - ref[0]), e1 = exp2f(s[nb][1] - ref[0]);
-                    const float e2 = exp2f(s[nb][2] - ref[1]), e3 = exp2f(s[nb][3] - ref[1]);
+                for (int nb = 0; nb < 4; ++nb) {
+                    const float e0 = ex2_approx(s[nb][0] - ref[0]), e1 = ex2_approx(s[nb][1] - ref[0]);
+                    const float e2 = ex2_approx(s[nb][2] - ref[1]), e3 = ex2_approx(s[nb][3] - ref[1]);
                     l_run[0] += e0 + e1; l_run[1] += e2 + e3;
                     pf[nb][0] = pack_h2(e0, e1); pf[nb][1] = pack_h2(e2, e3);        // the one rounding of a weight, as the product takes it
                 }
-                const int vr = wk * 16 + (lane & 15);
-                const uint8_t* vrow = vs_ + vr * 128;
                 #pragma unroll
-                for (int db = 0; db < 16; db += 2) {
-                    const int ch = db + (lane >> 4);
-                    uint32_t b0, b1, b2, b3;
-                    ldsm_x4_t(b0, b1, b2, b3, vrow + (ch >> 3) * Cfg::HALF + (((ch & 7) ^ (vr & 7)) << 4));
-                    if (!clear) { b0 &= keep[0]; b1 &= keep[1]; b2 &= keep[0]; b3 &= keep[1]; }
-                    mma_f16(o_acc[db], pf[0][0], pf[0][1], pf[1][0], pf[1][1], b0, b1);
-                    mma_f16(o_acc[db + 1], pf[0][0], pf[0][1], pf[1][0], pf[1][1], b2, b3);
+                for (int tile = 0; tile < 2; ++tile) {
+                    if (tile) values(1);
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        if (!clear) { vf[x][0] &= keep[2 * tile]; vf[x][1] &= keep[2 * tile + 1]; vf[x][2] &= keep[2 * tile]; vf[x][3] &= keep[2 * tile + 1]; }
+                        mma_f16(o_acc[2 * x], pf[2 * tile][0], pf[2 * tile][1], pf[2 * tile + 1][0], pf[2 * tile + 1][1], vf[x][0], vf[x][1]);
+                        mma_f16(o_acc[2 * x + 1], pf[2 * tile][0], pf[2 * tile][1], pf[2 * tile + 1][0], pf[2 * tile + 1][1], vf[x][2], vf[x][3]);
+                    }
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[stage]);
+            if (lane == 0) { mbar_arrive(&empty[st0]); if (two) mbar_arrive(&empty[st1]); }
+            it += two ? 2 : 1;
         }
         if (!ok) break;
 

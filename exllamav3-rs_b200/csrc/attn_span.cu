@@ -89,7 +89,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
     if (Cfg::KW == 1) { maps.k16 = maps.k; maps.v16 = maps.v; }
     static bool done[64] = {};
     if (!span_configure(attn_rows_kernel<HW>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
-    const int ctas = 2 * ctx->num_sms;
+    const int ctas = ctx->num_sms;
     ArParams p;
     p.a = a;
     p.min_share = AR_MIN_KEYS / Cfg::TK;
@@ -145,7 +145,7 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     if (groups) p.rest = (float*)exl3_ws_take(ctx, &off, place);
     float* own = any_long ? (float*)exl3_ws_take(ctx, &off, (size_t)2 * ctx->num_sms * 2 * AS_BLOCK * SPAN_PART * 4) : nullptr;
     size_t probe = off;
-    if (!share || (groups && (!prefix || !p.rest)) || (any_long && !own) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)4 * ctx->num_sms * AR_SCRATCH)))
+    if (!share || (groups && (!prefix || !p.rest)) || (any_long && !own) || (any_few && !exl3_ws_take(ctx, &probe, (size_t)2 * ctx->num_sms * AR_SCRATCH)))
         return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     int rc = EXL3_OK;
     if (groups) {

@@ -443,21 +443,19 @@ class Ctx:
             return shape[0], shape[0] if max_q_len is None else max_q_len, shape[1]
         raise Exl3Error(f"{what}: shape mismatch")
 
-    def _rope_append(self, q, k, v, planes, bits, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm,
+    def _rope_append(self, q, k, v, shape, pages, planes, bits, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm,
                      k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream, what):
         f16, i32 = torch.float16, torch.int32
         _chk(k, f16, "k"); _chk(v, f16, "v"); _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens")
-        shape, table, n_freq, nq = k.shape, block_table.shape, 0, 0
-        bsz, hd = table[0], shape[-1]
+        n_freq, nq, n_axes, hd = 0, 0, 1, shape[-1]
+        bsz, pps = block_table.shape
         rows, seq, nkv = self._packed(shape, cu_q, max_q_len, bsz, what)
-        pages, page = planes[0].shape[:2]
-        good = v.shape == shape and cache_seqlens.numel() == bsz and page == 256 and k.get_device() == self.device
-        n_axes = 1
+        good = v.shape == shape and cache_seqlens.numel() == bsz and k.get_device() == self.device
         if q is not None:
             _chk(q, f16, "q")
             full = q.shape
             nq = full[-2]
-            good = good and full[:-2] == shape[:-2] and full[-1] == hd
+            good = good and len(full) == len(shape) and full[0] == shape[0] and full[-1] == hd and (cu_q is not None or full[1] == seq)
             if out_q is not None:
                 _chk(out_q, f16, "out_q")
                 good = good and out_q.shape == full
@@ -483,7 +481,7 @@ class Ctx:
         args = _ROPE_APPEND.pack(_num(q), _num(out_q), k.data_ptr(), v.data_ptr(), _num(inv_freq), _num(positions), _num(q_norm), _num(k_norm),
                                  planes[0].data_ptr(), planes[1].data_ptr(), _num(planes[2]), _num(planes[3]), block_table.data_ptr(),
                                  cache_seqlens.data_ptr(), _num(cu_q), norm_eps, norm_constant_bias, attn_factor, n_freq, n_axes, rope_mode, bsz,
-                                 seq, rows, nq, nkv, hd, pages, table[1], bits[0], bits[1], freq_axis or b"")
+                                 seq, rows, nq, nkv, hd, pages, pps, bits[0], bits[1], freq_axis or b"")
         rc = lib().exl3_rope_append_paged(self._h, self._stream(stream), args)
         if rc:
             self.check(rc, what)
@@ -494,10 +492,10 @@ class Ctx:
         """Head norm and rotation of q and k, k and v into the fp16 pools, one launch.  positions: None, int32 [rows] or
         [axes, rows]; freq_axis: the axis of every frequency (bytes, or a list of them).  out_q None: q in place."""
         _chk(k_cache, torch.float16, "k_cache"); _chk(v_cache, torch.float16, "v_cache")
-        shape = k_cache.shape
-        if shape[2:] != k.shape[-2:] or v_cache.shape != shape:
+        cache, shape = k_cache.shape, k.shape
+        if len(cache) != 4 or cache[1] != 256 or cache[2] != shape[-2] or cache[3] != shape[-1] or v_cache.shape != cache:
             raise Exl3Error("rope_append_paged: the pools must be [pages, 256, nkv, head_dim]")
-        self._rope_append(q, k, v, (k_cache, v_cache, None, None), (0, 0), block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions,
+        self._rope_append(q, k, v, shape, cache[0], (k_cache, v_cache, None, None), (0, 0), block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions,
                           freq_axis, q_norm, k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream, "rope_append_paged")
 
     def rope_append_paged_q(self, q, k, v, qk, sk, qv, sv, block_table, cache_seqlens, inv_freq, out_q=None, cu_q=None, max_q_len=None,
@@ -506,10 +504,10 @@ class Ctx:
         """The same into the quantised pools (qk/qv int32 [pages,256,groups*bits], sk/sv fp16 [pages,256,groups])."""
         _chk(qk, torch.int32, "qk"); _chk(qv, torch.int32, "qv"); _chk(sk, torch.float16, "sk"); _chk(sv, torch.float16, "sv")
         groups = k.shape[-2] * k.shape[-1] // 32
-        if (sk.shape[2:] != (groups,) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
+        if (sk.shape[1:] != (256, groups) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
                 qk.shape[2] % groups or qv.shape[2] % groups or not qk.shape[2] or not qv.shape[2]):
             raise Exl3Error("rope_append_paged_q: the pools do not have the heads of k")
-        self._rope_append(q, k, v, (qk, qv, sk, sv), (qk.shape[2] // groups, qv.shape[2] // groups), block_table, cache_seqlens, inv_freq, out_q,
+        self._rope_append(q, k, v, k.shape, sk.shape[0], (qk, qv, sk, sv), (qk.shape[2] // groups, qv.shape[2] // groups), block_table, cache_seqlens, inv_freq, out_q,
                           cu_q, max_q_len, positions, freq_axis, q_norm, k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream,
                           "rope_append_paged_q")
 
