@@ -26,6 +26,7 @@ constexpr int AR_THREADS = (AR_WARPS + 1) * 32;
 constexpr int AR_STAGE = 32768;                         // keys and values of a tile
 constexpr int AR_MS = SPAN_PART;
 constexpr int AR_MAX_BSZ = 1024;                        // sequences of a launch: their tile counts are summed in shared memory
+constexpr int AR_SNAP = 6;                              // a part ends with a unit that would end so many tiles from there
 constexpr int AR_UNITS = AR_STAGES + 1;                 // unit descriptors: the producer is at most AR_STAGES tiles, so units, ahead
 
 struct ArUnit { int b, hg, row_base, ql, cached, key_lo, group, whole, slot, c0, pieces, tiles; };
@@ -46,6 +47,8 @@ struct ArCfg {
     static_assert(BYTES + 1024 + 64 <= EXL3_SM_SMEM, "a CTA per SM");
     static_assert(OFF_ML % 8 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
+
+template <int N> struct ArInt { static constexpr int value = N; };
 
 struct ArMaps { CUtensorMap k, v, k16, v16; };          // boxes of a tile, and of 16 tokens of one half of one head
 
@@ -114,29 +117,47 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
         if (lane == 0) sum[p.bsz] = before;
     }
     __syncthreads();
-    // this CTA's part [f0, f1) of the line of all tiles: sequence, head group, tile
+    // this CTA's part [f0, f1) of the line of all tiles: sequence, head group, tile.  (A 64-bit division is a quarter of a microsecond of every
+    // CTA's start: what fits in 32 bits is divided there.)
+    auto quotient = [](long long x, int y) -> long long { return x >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y); };
     const long long F = (long long)sum[p.bsz] * n_hg;
-    const long long want = (F + p.min_share - 1) / p.min_share;
-    const int C = (int)min((long long)gridDim.x, max(want, 1LL));
-    const int c = blockIdx.x;
-    const long long f0 = c < C ? c * F / C : F, f1 = c < C ? (c + 1) * F / C : F;
+    const long long share = max(quotient(F + gridDim.x - 1, gridDim.x), (long long)p.min_share);
+    const int c = blockIdx.x, snap = (int)min((long long)AR_SNAP, share / 4);
+    auto sequence_of = [&](long long f) -> int {            // the one with tile f: sum[b] * n_hg <= f < sum[b + 1] * n_hg
+        const long long per_group = quotient(f, n_hg);
+        int lo = 0, hi = p.bsz;
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (sum[mid] <= per_group) lo = mid; else hi = mid; }
+        return lo;
+    };
+    // Where part c begins.  A cut unit costs some 5 us, its partial sums' way through memory: parts end with a unit that ends near by.
+    auto begin_of = [&](int c) -> long long {
+        const long long f = c * share;
+        if (c == 0 || f >= F) return min(f, F);
+        const int b = sequence_of(f), n = sum[b + 1] - sum[b];
+        const long long in = f - (long long)sum[b] * n_hg;
+        const int from = (int)(in - quotient(in, n) * n);
+        return from <= snap && from <= n - from ? f - from : n - from <= snap ? f + (n - from) : f;
+    };
+    const long long begins = begin_of(c + (lane & 1));      // side by side
+    const long long f0 = __shfl_sync(0xffffffffu, begins, 0), f1 = __shfl_sync(0xffffffffu, begins, 1);
     if (f0 >= f1) {
         if (!p.first) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
-    auto cta_of = [&](long long f) -> int { return (int)(((f + 1) * C - 1) / F); };
+    // the last parts that do not begin behind a unit's first and last tile: the two parts around each, and itself, side by side
+    auto parts_of = [&](long long first, long long last, int& c0, int& c1) {
+        const long long f = lane & 4 ? last : first;
+        const int k = (int)(share >> 31 ? f / share : quotient(f, (int)share)) - 1 + (lane & 3);
+        const unsigned in = __ballot_sync(0xffffffffu, (lane & 3) < 3 && k >= 0 && begin_of(k) <= f);
+        c0 = __shfl_sync(0xffffffffu, k, 31 - __clz(in & 0x0fu));
+        c1 = __shfl_sync(0xffffffffu, k, 31 - __clz(in & 0xf0u));
+    };
 
     if (warp == AR_WARPS) {
         // ===== producer: the whole warp walks, lane 0 issues; lane i holds the block table's entry page0 + i
         int it = 0, n_unit = 0;
         long long f = f0;
-        int b = 0;
-        {
-            const int per_group = (int)(f0 / n_hg);     // last sequence whose first tile is not behind f0: sum[b] * n_hg <= f0
-            int lo = 0, hi = p.bsz;
-            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (sum[mid] <= per_group) lo = mid; else hi = mid; }
-            b = lo;
-        }
+        int b = sequence_of(f0);
         bool ok = true;
         SpanSeq s = {0, 0, 0};
         SpanTiles t = {};
@@ -145,7 +166,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
         while (f < f1 && ok) {
             while ((long long)sum[b + 1] * n_hg <= f) ++b;
             const int n = sum[b + 1] - sum[b];
-            const int in = (int)(f - (long long)sum[b] * n_hg), hg = in / n, from = in - hg * n;
+            const long long in = f - (long long)sum[b] * n_hg;
+            const int hg = (int)quotient(in, n), from = (int)(in - (long long)hg * n);
             const int upto = (int)min((long long)n, from + (f1 - f));
             const int gb = p.b0 + b;
             const int32_t* bt = a.block_table + (size_t)gb * a.pps;
@@ -167,13 +189,18 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                     if (page >= a.pages) page = -1;
                 }
                 if (it >= AR_STAGES && !mbar_wait_sleep_warp(&empty[stage], ((it / AR_STAGES) - 1) & 1)) { ok = false; break; }
+                // what a cut unit's partial sums need is found under the copies of its tiles, and read behind the last one
+                const bool cut = i == upto - 1 && !(from == 0 && upto == n);
+                int c0 = 0, c1 = 0;
+                if (cut) parts_of(u0, u0 + n - 1, c0, c1);
                 if (lane == 0) {
+                    if (cut) { units[n_unit % AR_UNITS].c0 = c0; units[n_unit % AR_UNITS].pieces = c1 - c0 + 1; }
                     if (i == from) {
                         ArUnit& u = units[n_unit % AR_UNITS];
                         u.b = gb; u.hg = hg; u.row_base = s.row_base; u.ql = s.ql; u.cached = s.cached; u.key_lo = grp.len; u.group = grp.g;
                         u.whole = from == 0 && upto == n;
                         u.slot = 2 * c + (from == 0 ? 1 : 0);
-                        u.c0 = cta_of(u0); u.pieces = cta_of(u0 + n - 1) - u.c0 + 1; u.tiles = upto - from;
+                        u.tiles = upto - from;
                     }
                     tile_of[stage] = page < 0 ? -1 : kt;
                     if (page < 0) mbar_arrive(&full[stage]);
@@ -227,7 +254,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     int it = 0, n_unit = 0;
     for (long long f = f0; f < f1 && ok; ++n_unit) {
         if (!mbar_wait_warp(&full[it % AR_STAGES], (it / AR_STAGES) & 1)) { ok = false; break; }
-        const ArUnit u = units[n_unit % AR_UNITS];
+        ArUnit u = units[n_unit % AR_UNITS];
         f += u.tiles;
         const int n_rows = u.ql * G, kvh = u.hg * HW + wh;
         int lo[2], hi[2];
@@ -352,6 +379,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
             it += two ? 2 : 1;
         }
         if (!ok) break;
+        if (!u.whole) { const volatile ArUnit& v = units[n_unit % AR_UNITS]; u.c0 = v.c0; u.pieces = v.pieces; }
 
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -393,15 +421,18 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
             }
             if (__shfl_sync(0xffffffffu, before, 0) != u.pieces - 1) continue;
             __threadfence();
-            constexpr int U = 4;
-            for (int r0 = 0; r0 < n_rows; r0 += U) {
-                SpanSum sums[U];
-                span_merge(sums, u.pieces, [&](int k, int i) -> const float* { return part(k, min(r0 + i, n_rows - 1)); },
-                           [](int, int) { return true; }, lane);
-                #pragma unroll
-                for (int i = 0; i < U; ++i)
-                    if (r0 + i < n_rows) span_put(a, p.rest, u.group, place(r0 + i), sums[i], lane);
-            }
+            auto join = [&](auto rows_at_once, auto ahead) {
+                constexpr int U = decltype(rows_at_once)::value;
+                for (int r0 = 0; r0 < n_rows; r0 += U) {
+                    SpanSum sums[U];
+                    span_merge<decltype(ahead)::value>(sums, u.pieces, [&](int k, int i) -> const float* { return part(k, min(r0 + i, n_rows - 1)); },
+                                                       [](int, int) { return true; }, lane);
+                    #pragma unroll
+                    for (int i = 0; i < U; ++i)
+                        if (r0 + i < n_rows) span_put(a, p.rest, u.group, place(r0 + i), sums[i], lane);
+                }
+            };
+            if (u.pieces <= 2) join(ArInt<8>(), ArInt<2>()); else join(ArInt<4>(), ArInt<4>());
         } else {
             // ---- the sums of the warps of a head: a common maximum, then one warp after the other adds to the buffer
             float* merge = reinterpret_cast<float*>(smem + Cfg::OFF_MERGE) + wh * AR_ROWS * AR_MS;
@@ -475,7 +506,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                             if (row(i) < n_rows) sums[i] = {reinterpret_cast<const float4*>(at)[lane], at[128], at[129]};
                         }
                     } else
-                        span_merge(sums, u.pieces, [&](int k, int i) -> const float* { return part(k, min(row(i), n_rows - 1)); },
+                        span_merge<4>(sums, u.pieces, [&](int k, int i) -> const float* { return part(k, min(row(i), n_rows - 1)); },
                                    [](int, int) { return true; }, lane);
                     #pragma unroll
                     for (int i = 0; i < 4; ++i)

@@ -81,13 +81,12 @@ __device__ __forceinline__ int span_places(int tiles, int share) { return share 
 
 // Sums of U rows over n parts each.  A warp; lane = four dims, all lanes have top and l.  part(k, u): part k of row u,
 // there(k, u): whether the row has it.  What waits for memory
-// is asked for together: the maxima and sums of all parts, and the values of four parts of every row, whatever the maxima are (a part
+// is asked for together: the maxima and sums of all parts, and the values of AHEAD parts of every row, whatever the maxima are (a part
 // without keys, or a place that nobody wrote values to, has weight 0 and is not looked at).  One after the other, 4 us per row.
 struct SpanSum { float4 acc; float top, l; };
-template <int U, typename Part, typename There>
+template <int AHEAD, int U, typename Part, typename There>
 __device__ __forceinline__ void span_merge(SpanSum (&s)[U], int n, Part part, There there, int lane)
 {
-    constexpr int AHEAD = 4;
     #pragma unroll
     for (int u = 0; u < U; ++u) s[u] = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
     for (int k0 = 0; k0 < n; k0 += 32) {
