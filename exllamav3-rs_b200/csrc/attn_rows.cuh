@@ -29,6 +29,8 @@ constexpr int AR_MAX_BSZ = 1024;                        // sequences of a launch
 constexpr int AR_SNAP = 6;                              // a part ends with a unit that would end so many tiles from there
 constexpr int AR_UNITS = AR_STAGES + 1;                 // unit descriptors: the producer is at most AR_STAGES tiles, so units, ahead
 
+constexpr int AR_PREFIX = 1 << 30;                      // bit of a tile that is read for a prefix
+
 struct ArUnit { int b, hg, row_base, ql, cached, key_lo, group, whole, slot, c0, pieces, tiles; };
 
 template <int HW>
@@ -60,6 +62,7 @@ struct ArParams {
     int* counters;                                      // [CTAs][4], zero between calls
     int* status;
     float* rest;                                        // [rows][nq][AR_MS] partial sums of sequences that a prefix is added to
+    int alone;                                          // prefixes are read here too, through their own table, by each sequence
     int first;                                          // nothing of this call is in front of the launch
 };
 
@@ -99,8 +102,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     auto tiles_of = [&](int b) -> int {
         const SpanSeq s = span_seq(a, b);
         if (s.ql == 0 || s.ql * G > AR_ROWS) return 0;
-        const SpanTiles t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, span_group(a, b, s.cached).len);
-        return max(t.sink + t.near, 1);
+        const int len = span_group(a, b, s.cached).len;
+        const SpanTiles t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, len);
+        return max((p.alone ? (len + TK - 1) / TK : 0) + t.sink + t.near, 1);
     };
     for (int b = tid; b < p.bsz; b += AR_THREADS) sum[b] = tiles_of(p.b0 + b);
     __syncthreads();
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
         SpanSeq s = {0, 0, 0};
         SpanTiles t = {};
         SpanGroup grp = {-1, 0, 0};
-        int have = -1, page0 = 0, entry = 0;
+        int have = -1, page0 = 0, entry = 0, n_pre = 0;
         while (f < f1 && ok) {
             while ((long long)sum[b + 1] * n_hg <= f) ++b;
             const int n = sum[b + 1] - sum[b];
@@ -170,17 +174,21 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
             const int hg = (int)quotient(in, n), from = (int)(in - (long long)hg * n);
             const int upto = (int)min((long long)n, from + (f1 - f));
             const int gb = p.b0 + b;
-            const int32_t* bt = a.block_table + (size_t)gb * a.pps;
             if (have != b) {
                 s = span_seq(a, gb);
                 grp = span_group(a, gb, s.cached);
                 t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, grp.len);
-                page0 = -64; have = b;
+                n_pre = p.alone ? (grp.len + TK - 1) / TK : 0;
+                have = b;
             }
+            page0 = -64;
             const long long u0 = f - from;
             for (int i = from; i < upto; ++i, ++it) {
                 const int stage = it % AR_STAGES;
-                const int kt = t.sink + t.near == 0 ? -1 : i < t.sink ? i : t.first + (i - t.sink);
+                const bool pre = i < n_pre;
+                const int own = i - n_pre, kt = pre ? i : t.sink + t.near == 0 ? -1 : own < t.sink ? own : t.first + (own - t.sink);
+                const int32_t* bt = a.block_table + (size_t)(pre ? grp.first : gb) * a.pps;
+                if (i == n_pre) page0 = -64;
                 int page = -1;
                 if (kt >= 0) {
                     const int pg = kt / PER_PAGE;
@@ -197,20 +205,20 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                     if (cut) { units[n_unit % AR_UNITS].c0 = c0; units[n_unit % AR_UNITS].pieces = c1 - c0 + 1; }
                     if (i == from) {
                         ArUnit& u = units[n_unit % AR_UNITS];
-                        u.b = gb; u.hg = hg; u.row_base = s.row_base; u.ql = s.ql; u.cached = s.cached; u.key_lo = grp.len; u.group = grp.g;
+                        u.b = gb; u.hg = hg; u.row_base = s.row_base; u.ql = s.ql; u.cached = s.cached; u.key_lo = grp.len; u.group = p.alone ? -1 : grp.g;
                         u.whole = from == 0 && upto == n;
                         u.slot = 2 * c + (from == 0 ? 1 : 0);
                         u.tiles = upto - from;
                     }
-                    tile_of[stage] = page < 0 ? -1 : kt;
+                    tile_of[stage] = page < 0 ? -1 : pre ? kt | AR_PREFIX : kt;
                     if (page < 0) mbar_arrive(&full[stage]);
                     else {
                         // groups of 16 keys with one that some row sees
                         const int k0 = kt * TK, tok = k0 & (EXL3_PAGE - 1);
                         int g0 = 0, g1 = KW;
                         if constexpr (KW > 1) {
-                            const int hi = min(TK, (i < t.sink ? min(a.sinks, t.end) : t.end) - k0);
-                            const int lo = i < t.sink || a.sinks > k0 ? 0 : max(0, t.lo - k0);
+                            const int hi = min(TK, (pre ? grp.len : own < t.sink ? min(a.sinks, t.end) : t.end) - k0);
+                            const int lo = pre || own < t.sink || a.sinks > k0 ? 0 : max(0, t.lo - k0);
                             g0 = lo >> 4; g1 = (hi + 15) >> 4;
                         }
                         uint8_t* st = smem + stage * AR_STAGE;
@@ -290,10 +298,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
             if (i > 0 && !mbar_wait_warp(&full[st0], (it / AR_STAGES) & 1)) { ok = false; break; }
             if (two && !mbar_wait_warp(&full[st1], ((it + 1) / AR_STAGES) & 1)) { ok = false; break; }
             const int kt0 = tile_of[st0], kt1 = two ? tile_of[st1] : -1;
-            const int kb0 = kt0 * TK + wk * 16, kb1 = kt1 * TK + wk * 16;            // first key of this warp's in either
-            auto seen = [&](int kt, int kb) { return kt >= 0 && kb < any_hi && (kb + 16 > any_lo || kb < a.sinks); };
-            auto whole = [&](int kt, int kb) { return kt >= 0 && kb + 16 <= all_hi && (kb >= all_lo || kb + 16 <= a.sinks); };
-            const bool in0 = seen(kt0, kb0), in1 = seen(kt1, kb1);
+            const bool pre0 = kt0 >= AR_PREFIX, pre1 = kt1 >= AR_PREFIX;             // of a prefix: every row sees all of it
+            const int kb0 = (kt0 & (AR_PREFIX - 1)) * TK + wk * 16, kb1 = (kt1 & (AR_PREFIX - 1)) * TK + wk * 16;     // first key of this warp's in either
+            auto seen = [&](int kt, int kb, bool pre) { return kt >= 0 && (pre ? kb < u.key_lo : kb < any_hi && (kb + 16 > any_lo || kb < a.sinks)); };
+            auto whole = [&](int kt, int kb, bool pre) { return kt >= 0 && (pre ? kb + 16 <= u.key_lo : kb + 16 <= all_hi && (kb >= all_lo || kb + 16 <= a.sinks)); };
+            const bool in0 = seen(kt0, kb0, pre0), in1 = seen(kt1, kb1, pre1);
             if (in0 || in1) {
                 const uint8_t* base[2] = {smem + st0 * AR_STAGE + wh * Cfg::HEAD, smem + st1 * AR_STAGE + wh * Cfg::HEAD};
                 float s[4][4];                                                      // blocks of 8 keys, two of either tile
@@ -323,7 +332,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                     }
                 };
                 values(0);
-                const bool clear = whole(kt0, kb0) && whole(kt1, kb1);              // every row sees every key of both
+                const bool clear = whole(kt0, kb0, pre0) && whole(kt1, kb1, pre1);              // every row sees every key of both
                 uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};      // values of keys that some row sees: pairs 2 t4, + 1 and 8 on
                 float mx[2] = {-INFINITY, -INFINITY};
                 #pragma unroll
@@ -333,9 +342,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                         float v = s[nb][e] * a.scale_log2;
                         if (!clear) {
                             const int key = (nb < 2 ? kb0 : kb1) + (nb & 1) * 8 + 2 * t4 + (e & 1), h = e >> 1;
-                            const bool in = nb < 2 ? in0 : in1;
-                            if (!(in && key < hi[h] && (key >= lo[h] || key < a.sinks))) v = -INFINITY;
-                            if (!(in && key < any_hi && (key >= any_lo || key < a.sinks))) keep[nb] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                            const bool in = nb < 2 ? in0 : in1, pre = nb < 2 ? pre0 : pre1;
+                            if (!(in && (pre ? key < u.key_lo : key < hi[h] && (key >= lo[h] || key < a.sinks)))) v = -INFINITY;
+                            if (!(in && (pre ? key < u.key_lo : key < any_hi && (key >= any_lo || key < a.sinks)))) keep[nb] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
                         }
                         s[nb][e] = v;
                         mx[e >> 1] = fmaxf(mx[e >> 1], v);

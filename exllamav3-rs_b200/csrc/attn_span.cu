@@ -75,11 +75,11 @@ bool span_configure(Kern kern, int bytes, int device, bool (&done)[64])
 
 // the sequences of few rows, HW heads side by side
 constexpr size_t AR_SCRATCH = (size_t)AR_WARPS * AR_ROWS * AR_MS * 4;       // per CTA and place, at most
-#ifndef AR_MIN_KEYS
-#define AR_MIN_KEYS 128
-#endif
+// Keys that a CTA takes at least: fewer are more partial sums to join (us at 64, 128 and 192 keys: one row over a window of 1024 16.2, 15.5 and
+// 20.7, of 4096 26, 20 and 23)
+constexpr int AR_MIN_KEYS = 128;
 template <int HW>
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, const AsParams& pre, size_t* ws_off)
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool alone, const AsParams& pre, size_t* ws_off)
 {
     using Cfg = ArCfg<HW>;
     ArMaps maps;
@@ -96,13 +96,13 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, con
     p.partial = (float*)exl3_ws_take(ctx, ws_off, 2 * ctas * AR_SCRATCH);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
-    p.rest = pre.rest;
+    p.rest = pre.rest; p.alone = alone;
     for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
         p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
         // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
         const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
-                                        ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1);
+                                        ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1) + 1;
         const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
         if (p.first) exl3_launch_first(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
         else exl3_launch(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
@@ -131,7 +131,12 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     if (span_empty(a)) return EXL3_OK;
     const int G = a.nq / a.nkv;
     const long long packed = (long long)a.q_len * G, all = (long long)a.rows * G;
-    const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long), groups = a.n_groups > 0;
+    const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long);
+    // A few sequences of few rows read a short prefix sooner each than together, which is two kernels more: up to 128 MB read again (as far as the
+    // host knows, from the table's width).  us, each and together, 16 / 8 heads, sequences x prefix: 4 x 512 18 and 30, 8 x 2048 24 and 32,
+    // 16 x 2048 36 and 39, 32 x 1024 37 and 34; 40 / 8 heads: 4 x 8192 41 and 44, 8 x 8192 59 and 46.
+    const bool alone = a.n_groups > 0 && !any_long && (long long)(a.bsz - 1) * a.pps * EXL3_PAGE * a.nkv * 512 <= 128LL << 20;
+    const bool groups = a.n_groups > 0 && !alone;
     // Two row blocks share the tiles where a group or a sequence may have that many rows
     const bool two_prefix = all > (long long)AS_BLOCK * a.n_groups, two_own = packed > AS_BLOCK;
     // Scratch.  Prefixes: a place per row, head and part, as many parts as a quarter of the scratch has room for, and one for
@@ -163,12 +168,14 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     }
     exl3_chain_scope behind(ctx, any_long);
     if (any_few) {
-        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, p, &off) : span_rows<1>(ctx, st, a, p.first != 0, p, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, alone, p, &off) : span_rows<1>(ctx, st, a, p.first != 0, alone, p, &off);
         if (rc) return rc;
     }
     if (groups) {
         const SpanJoinParams j = {a, prefix, share, p.rest};
-        exl3_launch(ctx, span_join_kernel, (unsigned)(((long long)a.rows * a.nq + 31) / 32), 256, 0, st, j);
+        const long long pairs = (long long)a.rows * a.nq;
+        if (pairs <= 64LL * ctx->num_sms) exl3_launch(ctx, span_join_kernel<1>, (unsigned)((pairs + 7) / 8), 256, 0, st, j);
+        else exl3_launch(ctx, span_join_kernel<4>, (unsigned)((pairs + 31) / 32), 256, 0, st, j);
         ctx->launches++;
     }
     return exl3_check_launch(ctx, what);

@@ -44,12 +44,16 @@ __device__ __forceinline__ SpanGroup span_group(const SpanArgs& a, int b, int ca
 {
     SpanGroup r = {-1, b, 0};
     if (a.n_groups == 0) return r;
-    int lo = 0, hi = a.n_groups;                  // group_start[lo] <= b
-    if (a.group_start[0] > b || a.group_start[hi] <= b) return r;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.group_start[mid] <= b) lo = mid; else hi = mid; }
-    const int len = min(a.prefix_lens[lo], a.pps * EXL3_PAGE);
+    int lo = 0, hi = a.n_groups;                  // group_start[lo] <= b < group_start[hi]
+    int from = a.group_start[0], len = a.prefix_lens[0];        // asked for together with the end: one group is the common case
+    if (from > b || a.group_start[hi] <= b) return r;
+    if (hi > 1) {
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (a.group_start[mid] <= b) lo = mid; else hi = mid; }
+        from = a.group_start[lo]; len = a.prefix_lens[lo];
+    }
+    len = min(len, a.pps * EXL3_PAGE);
     if (len <= 0 || len > cached) return r;
-    r.g = lo; r.first = max(a.group_start[lo], 0); r.len = len;
+    r.g = lo; r.first = max(from, 0); r.len = len;
     return r;
 }
 

@@ -678,11 +678,12 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     if (tid == 0 && s_failed) atomicExch(p.status, 3);
 }
 
-// Adds the partial sums of its prefix to every row of a sequence that has one: a warp takes four (row, head) pairs.
+// Adds the partial sums of its prefix to every row of a sequence that has one: a warp takes U (row, head) pairs, four where there are many,
+// and one where one each leaves SMs idle: then what counts is how often a warp waits for memory.
 struct SpanJoinParams { SpanArgs a; const float* prefix; const int* share; const float* rest; };
+template <int U>
 __global__ void __launch_bounds__(256) span_join_kernel(const SpanJoinParams p)
 {
-    constexpr int U = 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const SpanArgs& a = p.a;
     const int lane = threadIdx.x & 31;
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(256) span_join_kernel(const SpanJoinParams p)
     for (int u = 0; u < U; ++u) if (len[u]) places = max(places, span_places((len[u] + AS_TK - 1) / AS_TK, share));
     SpanSum sum[U];
     // place 0 of the sum is the sequence's own part; a place behind a shorter prefix's last stands for that one with weight 0
-    span_merge<4>(sum, places + 1, [&](int k, int u) -> const float* {
+    span_merge<U == 1 ? 12 : 4>(sum, places + 1, [&](int k, int u) -> const float* {
         const long long at = min(w0 + u, n - 1);
         return k == 0 ? p.rest + at * SPAN_PART : p.prefix + ((size_t)(k - 1) * n + at) * SPAN_PART;
     }, [&](int k, int u) -> bool { return k == 0 || k - 1 < (len[u] ? span_places((len[u] + AS_TK - 1) / AS_TK, share) : 0); }, lane);

@@ -20,7 +20,7 @@ class Batch:
     without a visible key are `unused`."""
 
     def __init__(self, q_lens, cached, nq, nkv, window=BIG, sinks=0, groups=None, prefix=None, copies=False, seed=0, extra_rows=0, unused=-1, q_std=1.5,
-                 pages=None, drop=()):
+                 pages=None, drop=(), width=0):
         import torch
         g = torch.Generator(device="cuda").manual_seed(seed)
         r = np.random.default_rng(seed)
@@ -28,7 +28,7 @@ class Batch:
         self.groups, self.prefix = groups, prefix
         bsz = len(q_lens)
         total = [c + x for c, x in zip(cached, q_lens)]
-        width = max(max((t + PAGE - 1) // PAGE for t in total), 1, *[(p + PAGE - 1) // PAGE for p in (prefix or [0])])
+        width = max(max((t + PAGE - 1) // PAGE for t in total), 1, width, *[(p + PAGE - 1) // PAGE for p in (prefix or [0])])
         self.seen = [np.zeros(width * PAGE, bool) for _ in range(bsz)]         # positions that some row sees
         for b, (x, c) in enumerate(zip(q_lens, cached)):
             for p in range(c, c + x):
@@ -271,11 +271,15 @@ PREFIXES = [
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [0, 9000])
 @pytest.mark.parametrize("copies", [False, True])
 @pytest.mark.parametrize("case", range(len(PREFIXES)))
-def test_prefix_shapes(ctx, case, copies):
+def test_prefix_shapes(ctx, case, copies, width):
+    """narrow tables, of which a few sequences read a prefix each, and wide ones, which may hold long prefixes"""
     q_lens, cached, nq, nkv, groups, lens = PREFIXES[case]
-    b = Batch(q_lens, cached, nq, nkv, groups=groups, prefix=lens, copies=copies, seed=case, extra_rows=2)
+    if width and len(q_lens) > 100:
+        width = 500
+    b = Batch(q_lens, cached, nq, nkv, groups=groups, prefix=lens, copies=copies, seed=case, extra_rows=2, width=width)
     b.check(prefix(ctx, b))
 
 
