@@ -1,5 +1,6 @@
 // exl3_window_attn_paged and exl3_prefix_attn_paged: attention over spans of the paged cache.
 #include <algorithm>
+#include <cmath>
 #include <limits.h>
 #include <math.h>
 #include "attn_span_tc.cuh"
@@ -79,7 +80,7 @@ constexpr size_t AR_SCRATCH = (size_t)AR_WARPS * AR_ROWS * AR_MS * 4;       // p
 // 20.7, of 4096 26, 20 and 23)
 constexpr int AR_MIN_KEYS = 128;
 template <int HW>
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool alone, const AsParams& pre, size_t* ws_off)
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool alone, bool plain, const AsParams& pre, int sms, size_t* ws_off)
 {
     using Cfg = ArCfg<HW>;
     ArMaps maps;
@@ -89,7 +90,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
     if (Cfg::KW == 1) { maps.k16 = maps.k; maps.v16 = maps.v; }
     static bool done[64] = {};
     if (!span_configure(attn_rows_kernel<HW>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
-    const int ctas = ctx->num_sms;
+    const int ctas = sms;
     ArParams p;
     p.a = a;
     p.min_share = AR_MIN_KEYS / Cfg::TK;
@@ -104,7 +105,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
                                         ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1) + 1;
         const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
-        if (p.first) exl3_launch_first(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
+        if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
         else exl3_launch(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
         ctx->launches++;
     }
@@ -113,17 +114,31 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
 
 // a launch of the tcgen05 kernel with NB row blocks per CTA
 template <int NB>
-int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p)
+int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p, int sms)
 {
     CUtensorMap kmap, vmap;
     if (!span_map(p.a, p.a.kc, AS_TK, 2, 1, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, 1, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     static bool done[64] = {};
     if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
-    const int grid = AsCfg<NB>::CTAS * ctx->num_sms;
+    const int grid = AsCfg<NB>::CTAS * sms;
     if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p);
     else exl3_launch(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p, 0);
     ctx->launches++;
     return EXL3_OK;
+}
+
+// SMs for the sequences of few rows beside those of many, from what the host knows of a batch over windows; 0: one after the other.  Long
+// sequences are at least so many as the rows need, and every one counts as full; a tile of 256 rows is 2.3 us, and an SM reads 42 GB/s.
+int span_aside(exl3_ctx* ctx, const SpanArgs& a)
+{
+    if (a.window > SPAN_MAX_LEN || a.q_len < 2) return 0;
+    const int G = a.nq / a.nkv;
+    const double keys = std::min((double)a.window + a.sinks, (double)a.pps * EXL3_PAGE);
+    const double n_long = std::max(0.0, std::ceil(((double)a.rows - a.bsz) / (a.q_len - 1))), n_few = a.bsz - n_long;
+    const double few = n_few * keys * a.nkv * 512 / 42e3;                                                  // us of one SM
+    const double many = n_long * std::ceil((double)a.q_len * G / 256) * a.nkv * (keys / AS_TK + 1.5) * 2.3;
+    if (n_long < 1 || n_few < 1 || few < many / 16 || many < few / 16 || few + many < 10.0 * ctx->num_sms) return 0;
+    return std::min(std::max((int)(ctx->num_sms * few / (few + many)), 8), ctx->num_sms - 8);
 }
 
 int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what)
@@ -155,20 +170,40 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     int rc = EXL3_OK;
     if (groups) {
         p.prefixes = 1; p.partial = prefix; p.share = share;
-        rc = two_prefix ? span_tc<2>(ctx, st, p) : span_tc<1>(ctx, st, p);
+        rc = two_prefix ? span_tc<2>(ctx, st, p, ctx->num_sms) : span_tc<1>(ctx, st, p, ctx->num_sms);
         if (rc) return rc;
         p.first = 0;
     }
     exl3_chain_scope chain(ctx, groups);
-    if (any_long) {
+    // Both classes of a batch over windows, where neither is small beside the other: each gets its share of the SMs, and the start and end of
+    // one kernel, 10 us and more, runs under the other (28 rows beside 4 x 251, window 1024: 104 us one after the other).
+    const int aside = any_long && any_few && !groups && a.n_groups == 0 ? span_aside(ctx, a) : 0;
+    if (aside) {
+        if (cudaEventRecord(ctx->ev_fork, st) != cudaSuccess || cudaStreamWaitEvent(ctx->aux_stream, ctx->ev_fork, 0) != cudaSuccess)
+            return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream fork failed");
+        const int chained = ctx->chain;
+        ctx->chain = 0;                                      // a plain launch: nothing of the second stream is in front
+        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, ctx->aux_stream, a, true, false, true, p, aside, &off)
+                            : span_rows<1>(ctx, ctx->aux_stream, a, true, false, true, p, aside, &off);
+        ctx->chain = chained;
+        ctx->chain_break = 1;
+    }
+    if (any_long && rc == EXL3_OK) {
         p.prefixes = 0; p.partial = own; p.share = share + 1;
-        rc = two_own ? span_tc<2>(ctx, st, p) : span_tc<1>(ctx, st, p);
-        if (rc) return rc;
+        rc = two_own ? span_tc<2>(ctx, st, p, ctx->num_sms - aside) : span_tc<1>(ctx, st, p, ctx->num_sms - aside);
         p.first = 0;
     }
+    if (aside) {
+        // joined after an error too, so that a capture in progress stays well-formed
+        if (cudaEventRecord(ctx->ev_join, ctx->aux_stream) != cudaSuccess || cudaStreamWaitEvent(st, ctx->ev_join, 0) != cudaSuccess)
+            return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream join failed");
+        return rc ? rc : exl3_check_launch(ctx, what);
+    }
+    if (rc) return rc;
     exl3_chain_scope behind(ctx, any_long);
     if (any_few) {
-        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, alone, p, &off) : span_rows<1>(ctx, st, a, p.first != 0, alone, p, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, alone, false, p, ctx->num_sms, &off)
+                            : span_rows<1>(ctx, st, a, p.first != 0, alone, false, p, ctx->num_sms, &off);
         if (rc) return rc;
     }
     if (groups) {

@@ -636,7 +636,38 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             }
             if (__shfl_sync(0xffffffffu, before, 0) != x.count - 1) continue;
             __threadfence();
-            // all parts of the unit are there: a thread per row
+            // all parts of the unit are there: a thread per row.  Of two, this one's is still in tensor memory, and the other one's values are asked for
+            // 32 columns ahead; each product is rounded before the sum, so that it does not matter which of the two is here.
+            if (x.count == 2) {
+                const float* other = own_part(1 - x.index);
+                float4 v[8];
+                auto fetch = [&](int c) {
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(other) + (c * 8 + i) * 32 + lane);
+                };
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(other + 32 * 128) + lane);
+                fetch(0);
+                const float top2 = fmaxf(m_used, y.x), ref2 = top2 == -INFINITY ? 0.f : top2;
+                const float w0 = exp2f(m_used - ref2), w1 = exp2f(y.x - ref2), l2 = __fadd_rn(__fmul_rn(l, w0), __fmul_rn(y.y, w1));
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float o[32];
+                    tc_ld32(to_ + c * 32, o);
+                    tc_wait_ld();
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        o[4 * i] = __fadd_rn(__fmul_rn(o[4 * i], w0), __fmul_rn(v[i].x, w1));
+                        o[4 * i + 1] = __fadd_rn(__fmul_rn(o[4 * i + 1], w0), __fmul_rn(v[i].y, w1));
+                        o[4 * i + 2] = __fadd_rn(__fmul_rn(o[4 * i + 2], w0), __fmul_rn(v[i].z, w1));
+                        o[4 * i + 3] = __fadd_rn(__fmul_rn(o[4 * i + 3], w0), __fmul_rn(v[i].w, w1));
+                    }
+                    if (c < 3) fetch(c + 1);
+                    if (x.group < 0) put_half(o, l2 > 0.f ? 1.0f / l2 : 0.f, c);
+                    else put_float(o, c);
+                }
+                if (x.group >= 0 && lane < n_mine) *reinterpret_cast<float2*>(by_row + row_of(lane) * SPAN_PART + 128) = make_float2(top2, l2);
+                continue;
+            }
             auto max_sum = [&](int k) -> float2 { return __ldcg(reinterpret_cast<const float2*>(own_part(k) + 32 * 128) + lane); };
             float top = -INFINITY, l_all = 0.f;
             #pragma unroll 4

@@ -168,6 +168,8 @@ WINDOWS = [
     ([1, 64, 1, 2, 333], [3000, 100, 5, 1500, 1], 256, 70, 32, 4), ([1, 1], [9000, 5], 8192, 300, 40, 8), ([300], [1000], 5000, 0, 16, 2),
     ([257], [255], 63, 1, 16, 8), ([129], [0], 129, 0, 5, 1), ([64, 64], [4096, 4095], 4096, 64, 16, 8), ([1] * 300, [20] * 300, 16, 2, 16, 8),
     ([2] * 1200, [30] * 1200, 16, 2, 16, 8),
+    # both classes large enough that they run side by side
+    ([1, 251, 1, 251] * 2 + [1] * 24, [600 + 137 * i for i in range(32)], 1024, 4, 40, 8), ([1] * 90 + [300] * 2, [5 * i for i in range(92)], 4096, 0, 9, 3),
 ]
 
 
@@ -334,6 +336,32 @@ def test_prefix_lengths_are_read_at_replay(ctx):
         torch.cuda.synchronize()
         b.check(b.o)
         w.check(w.o)
+
+
+@pytest.mark.gpu
+def test_classes_side_by_side_in_a_graph(ctx):
+    """a call that forks to a second stream and joins, captured and replayed, and eager calls right behind one another"""
+    import torch
+    import exl3b200
+    b = Batch([1] * 28 + [251] * 4, [600 + 137 * i for i in range(32)], 40, 8, 1024, 4, seed=12)
+    call = lambda s=None: ctx.window_attn_paged(b.q, b.k, b.v, b.bt, b.sl, b.o, 1024, sinks=4, cu_q=b.cu, max_q_len=251, stream=s)  # noqa: E731
+    for _ in range(5):
+        call()
+    b.check(b.o)
+    first = b.o.clone()
+    graph = exl3b200.CudaGraph(ctx)
+    torch.cuda.synchronize()
+    graph.capture_begin()
+    for _ in range(2):
+        call(graph.side_stream())
+    graph.capture_end()
+    for _ in range(3):
+        b.o.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(b.o, first)
+    ctx.poll_status()
 
 
 @pytest.mark.gpu
