@@ -21,6 +21,7 @@ int span_check(exl3_ctx* ctx, const SpanArgs& a, int hd, float sm_scale, const c
         return bad(EXL3_ERR_INVALID, "bad shape");
     if (!a.cu_q && (long long)a.bsz * a.q_len != a.rows) return bad(EXL3_ERR_INVALID, "rows must be bsz * q_len without cu_q");
     if (a.nq % a.nkv != 0) return bad(EXL3_ERR_INVALID, "n_q_heads must be a multiple of n_kv_heads");
+    if (a.nq / a.nkv > AS_BLOCK) return bad(EXL3_ERR_UNSUPPORTED, "more than 128 query heads per kv head");
     if (a.bsz > 32 * AS_MAX_CHUNKS) return bad(EXL3_ERR_UNSUPPORTED, "more than 8192 sequences");
     if ((long long)a.rows * a.nq > 1LL << 30) return bad(EXL3_ERR_INVALID, "too many rows");
     if (hd != 128) return bad(EXL3_ERR_UNSUPPORTED, "head_dim must be 128");
@@ -62,6 +63,20 @@ bool span_map(const SpanArgs& a, const void* pool, int tokens, int halves, int h
     cuuint32_t box[5] = {64, (cuuint32_t)tokens, (cuuint32_t)halves, (cuuint32_t)heads, 1};
     cuuint32_t one[5] = {1, 1, 1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The queries as {64 dims, 2 halves, heads, rows}: a box of a kv head's G heads and so many rows lands as packed rows
+bool span_q_map(const SpanArgs& a, int rows, CUtensorMap* map)
+{
+    EncodeTiledFn enc = span_encode_tiled();
+    if (!enc) return false;
+    const int G = a.nq / a.nkv;
+    cuuint64_t dims[4] = {64, 2, (cuuint64_t)a.nq, (cuuint64_t)a.rows};
+    cuuint64_t strides[3] = {128, 256, (cuuint64_t)a.nq * 256};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)G, (cuuint32_t)(rows / G)};
+    cuuint32_t one[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<half*>(a.q), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -116,13 +131,14 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
 template <int NB>
 int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p, int sms)
 {
-    CUtensorMap kmap, vmap;
-    if (!span_map(p.a, p.a.kc, AS_TK, 2, 1, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, 1, &vmap)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
+    CUtensorMap kmap, vmap, qmap;
+    if (!span_map(p.a, p.a.kc, AS_TK, 2, 1, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, 1, &vmap) || !span_q_map(p.a, AsCfg<NB>::ROWS, &qmap))
+        return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     static bool done[64] = {};
     if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int grid = AsCfg<NB>::CTAS * sms;
-    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p);
-    else exl3_launch(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, p, 0);
+    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p);
+    else exl3_launch(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p, 0);
     ctx->launches++;
     return EXL3_OK;
 }

@@ -43,11 +43,12 @@ template <int NB>
 struct AsCfg {
     static constexpr int ROWS = AS_BLOCK * NB, SW = 4 * NB, THREADS = (SW + 2) * 32;       // softmax warps, TMA producer, MMA issuer
     static constexpr int SLOTS = 2 * NB;                                                   // ring of tiles: K0 V0 K1 V1 ...
+    static constexpr int QHALF = ROWS * 128;                                               // Q: halves of a head, rows of 128 bytes
     static constexpr int OFF_KV = NB * AS_TILE, OFF_STAGE = OFF_KV + SLOTS * AS_TILE;      // Q in front; 2 KB per softmax warp
     static constexpr int OFF_PIECE = OFF_STAGE + SW * 2048;
     static constexpr int OFF_SUM = OFF_PIECE + 2 * (int)sizeof(AsPiece);
     static constexpr int OFF_BAR = OFF_SUM + (AS_MAX_CHUNKS + 2) * 4;
-    static constexpr int NBARS = 5 * NB + 2 * SLOTS + 4;                                   // q_full, s_full, p_half, p_full, o_full; full, empty per slot; piece full, empty
+    static constexpr int NBARS = 4 * NB + 2 * SLOTS + 6;                                   // s_full, p_half, p_full, o_full; full, empty per slot; piece full, empty; q full, empty
     static constexpr int SMEM = OFF_BAR + NBARS * 8 + 16 + 1024;
     static constexpr int CTAS = NB == 1 ? 2 : 1, TMEM = 256 * NB;
     static_assert(OFF_SUM % 8 == 0 && OFF_BAR % 8 == 0, "alignment of the barriers");
@@ -183,10 +184,11 @@ __device__ __forceinline__ float2 exp2_poly(float2 x)
 template <int NB>
 __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                                          const __grid_constant__ CUtensorMap vmap,
+                                                                                         const __grid_constant__ CUtensorMap qmap,
                                                                                          const AsParams p, int early)
 {
     using Cfg = AsCfg<NB>;
-    constexpr int SW = Cfg::SW, SLOTS = Cfg::SLOTS, ROWS = Cfg::ROWS;
+    constexpr int SW = Cfg::SW, SLOTS = Cfg::SLOTS;
     (void)early;
     pdl_wait();
     extern __shared__ uint8_t smem_unaligned[];
@@ -194,17 +196,19 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     AsPiece* pieces = reinterpret_cast<AsPiece*>(smem + Cfg::OFF_PIECE);
     int* sums = reinterpret_cast<int*>(smem + Cfg::OFF_SUM);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
-    uint64_t *q_full = bars, *s_full = q_full + NB, *p_half = s_full + NB, *p_full = p_half + NB, *o_full = p_full + NB, *kv_full = o_full + NB,
-             *kv_empty = kv_full + SLOTS, *piece_full = kv_empty + SLOTS, *piece_empty = piece_full + 2;
+    uint64_t *s_full = bars, *p_half = s_full + NB, *p_full = p_half + NB, *o_full = p_full + NB, *kv_full = o_full + NB,
+             *kv_empty = kv_full + SLOTS, *piece_full = kv_empty + SLOTS, *piece_empty = piece_full + 2, *q_full = piece_empty + 2, *q_empty = q_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NBARS);
     __shared__ int s_failed;
 
     const SpanArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.nq / a.nkv, n = p.prefixes ? a.n_groups : a.bsz, n_chunks = (n + 31) / 32;
+    const int rows = Cfg::ROWS / G * G;                     // of a unit: whole rows of the call, so that a copy places them as packed rows
     if (tid == 0) {
         s_failed = 0;
-        for (int i = 0; i < NB; ++i) { mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        for (int i = 0; i < NB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
         for (int i = 0; i < SLOTS; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], SW + 1); }
         mbar_fence_init();
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     int tiles = 0;
     for (int ch = (warp + 2) % (SW + 2); ch < n_chunks; ch += SW + 2) {
         AsEntry e;
-        const int own = as_entry_tiles(p, ch * 32, n, ROWS, G, lane, e);
+        const int own = as_entry_tiles(p, ch * 32, n, rows, G, lane, e);
         if (ch == 0) { mine = e; tiles = own; }
         int v = own;
         #pragma unroll
@@ -258,27 +262,27 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
 
     if (warp == SW) {
         // ===== producer: walks this CTA's part of the line; warp-uniform, lane 0 issues
-        int ch = 0, it = 0, n_piece = 0;
+        int ch = 0, it = 0, n_piece = 0, n_q = 0;
         long long f = f0, at = 0;                           // at: where the chunk, then the entry begins
         while ((long long)(sums[ch] * (long long)a.nkv) + at <= f) { at += sums[ch] * (long long)a.nkv; ++ch; }
-        if (ch > 0) tiles = as_entry_tiles(p, ch * 32, n, ROWS, G, lane, mine);
+        if (ch > 0) tiles = as_entry_tiles(p, ch * 32, n, rows, G, lane, mine);
         int j = 0;                                          // entry of the chunk
         auto seek = [&]() {                                  // entry j of the chunk that has f
             while (true) {
                 const long long w = (long long)__shfl_sync(0xffffffffu, tiles, j) * a.nkv;
                 if (at + w > f) return;
                 at += w;
-                if (++j == 32) { j = 0; ++ch; tiles = as_entry_tiles(p, ch * 32, n, ROWS, G, lane, mine); }
+                if (++j == 32) { j = 0; ++ch; tiles = as_entry_tiles(p, ch * 32, n, rows, G, lane, mine); }
             }
         };
         bool ok = true;
         while (f < f1 && ok) {
             seek();
             const AsEntry e = as_shfl(mine, j);
-            const int per_head = __shfl_sync(0xffffffffu, tiles, j), n_rb = as_blocks(e.n_rows, ROWS);
+            const int per_head = __shfl_sync(0xffffffffu, tiles, j), n_rb = as_blocks(e.n_rows, rows);
             int kvh = (int)((f - at) / per_head), in = (int)((f - at) - (long long)kvh * per_head), rb = 0;
             for (int b0 = 0;; b0 += 32) {                    // the row block that has tile `in` of the head
-                const int own = b0 + lane < n_rb ? as_count(p, e, b0 + lane, ROWS, G) : 0;
+                const int own = b0 + lane < n_rb ? as_count(p, e, b0 + lane, rows, G) : 0;
                 int v = own;
                 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += u; }
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             const long long end_e = at + (long long)per_head * a.nkv;
             // units of the entry, one after the other
             for (; f < min(f1, end_e) && ok; in = 0) {
-                const int r0 = rb * ROWS, r1 = min(r0 + ROWS, e.n_rows);
+                const int r0 = rb * rows, r1 = min(r0 + rows, e.n_rows);
                 const SpanTiles t = as_tiles(p, e, r0, r1, G);
                 const int total = max(t.sink + t.near, 1);
                 const long long u0 = f - in;
@@ -311,6 +315,13 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                         x.group = e.group;
                         mbar_arrive(&piece_full[n_piece & 1]);
                     }
+                    // Q, when the scores of the piece before are computed: two copies, one per half of the head
+                    if (n_piece > 0 && !mbar_wait_sleep_warp(q_empty, (n_piece - 1) & 1)) { ok = false; break; }
+                    if (lane == 0) {
+                        mbar_expect_tx(q_full, rows * 256);
+                        for (int h = 0; h < 2; ++h) tma_load_4d(smem + h * Cfg::QHALF, &qmap, 0, h, kvh * G, e.row_base + r0 / G, q_full);
+                    }
+                    ++n_q;
                     ++n_piece;
                     for (int k = in; k < in + take && ok; ++k) {
                         const int kt = k < t.sink ? k : t.first + (k - t.sink);
@@ -337,6 +348,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
         failed = !ok;
         // not out before every copy has landed, whatever became of those who take them
         for (int i = max(0, it - SLOTS); i < it; ++i) mbar_wait_sleep_warp(&kv_full[i % SLOTS], (i / SLOTS) & 1);
+        if (n_q > 0) mbar_wait_sleep_warp(q_full, (n_q - 1) & 1);
     } else if (warp == SW + 1) {
         // ===== MMA issuer: warp-uniform values, one elected lane
         const bool leader = elect_one();
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
         constexpr uint32_t LBO_K = 1u << 16, LBO_V = (uint32_t)((AS_TILE / 2) >> 4) << 16;
         auto mk = [](uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; };
         const uint32_t q_lo = (smem_u32(smem) >> 4) | LBO_K, kv_lo = smem_u32(smem + Cfg::OFF_KV) >> 4;
-        int done[2] = {0, 0}, begun[2] = {0, 0};                                          // tiles and pieces of each block
+        int done[2] = {0, 0};                                                             // tiles of each block
         for (int n_piece = 0; !failed; ++n_piece) {
             if (!mbar_wait_sleep_warp(&piece_full[n_piece & 1], (n_piece >> 1) & 1)) { failed = true; break; }
             const AsPiece& x = pieces[n_piece & 1];
@@ -353,27 +365,27 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             if (lane == 0) mbar_arrive(&piece_empty[n_piece & 1]);
             if (n_tiles == 0) break;
             // S of block b from the K tile that is ring item `item`
-            auto scores = [&](int b, int item) -> bool {
+            auto scores = [&](int b, int item, bool last) -> bool {
                 const int slot = item % SLOTS;
                 if (b == 0 && !mbar_wait_sleep_warp(&kv_full[slot], (item / SLOTS) & 1)) return false;
                 tc_fence_after();
                 if (leader) {
-                    const uint32_t qb = q_lo + b * (AS_TILE >> 4), kb = (kv_lo + slot * (AS_TILE >> 4)) | LBO_K;
+                    const uint32_t qb = q_lo + b * (AS_BLOCK * 128 >> 4), kb = (kv_lo + slot * (AS_TILE >> 4)) | LBO_K;
                     #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t off = ((kk >> 2) * (AS_TILE / 2) + (kk & 3) * 32) >> 4;
-                        tc_mma_f16(tmem + b * 256, mk(qb + off, HI), mk(kb + off, HI), ATC_IDESC_S, kk > 0 ? 1u : 0u);
+                        const uint32_t in = (kk & 3) * 32;
+                        tc_mma_f16(tmem + b * 256, mk(qb + (((kk >> 2) * Cfg::QHALF + in) >> 4), HI), mk(kb + (((kk >> 2) * (AS_TILE / 2) + in) >> 4), HI),
+                                   ATC_IDESC_S, kk > 0 ? 1u : 0u);
                     }
                     tc_commit(&s_full[b]);
-                    if (b == n_blocks - 1) tc_commit(&kv_empty[slot]);
+                    if (b == n_blocks - 1) { tc_commit(&kv_empty[slot]); if (last) tc_commit(q_empty); }
                 }
                 __syncwarp();
                 return true;
             };
-            for (int b = 0; b < n_blocks && !failed; ++b) {
-                if (!mbar_wait_sleep_warp(&q_full[b], begun[b] & 1) || !scores(b, ring)) failed = true;
-                ++begun[b];
-            }
+            if (!mbar_wait_warp(q_full, n_piece & 1)) { failed = true; break; }
+            for (int b = 0; b < n_blocks && !failed; ++b)
+                if (!scores(b, ring, n_tiles == 1)) failed = true;
             for (int j = 0; j < n_tiles && !failed; ++j) {
                 const int item = ring + 2 * j + 1, slot = item % SLOTS;
                 for (int b = 0; b < n_blocks && !failed; ++b) {
@@ -394,7 +406,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                     ++done[b];
                     if (failed) break;
                     // S of the next tile over P of this one: the tensor core runs the product before it first
-                    if (j + 1 < n_tiles) { if (!scores(b, item + 1)) failed = true; }
+                    if (j + 1 < n_tiles) { if (!scores(b, item + 1, j + 2 == n_tiles)) failed = true; }
                     else { if (leader) tc_commit(&o_full[b]); __syncwarp(); }
                 }
             }
@@ -406,6 +418,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
         const float scale = a.scale_log2;
         uint8_t* stage = smem + Cfg::OFF_STAGE + warp * 2048;
         int done = 0, begun = 0;                                            // tiles and pieces of this block
+        const int per8 = 8 / G, left8 = 8 - per8 * G;                       // rows and heads that 8 packed rows go on
         for (int n_piece = 0; !failed; ++n_piece) {
             if (!mbar_wait_warp(&piece_full[n_piece & 1], (n_piece >> 1) & 1)) { failed = true; break; }
             const AsPiece x = pieces[n_piece & 1];
@@ -413,30 +426,6 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             if (lane == 0) mbar_arrive(&piece_empty[n_piece & 1]);
             if (x.n_tiles == 0) break;
             if (blk * AS_BLOCK >= x.n_valid) continue;
-            {   // a warp's 32 Q rows -> shared memory, K-major, 128-byte swizzle: half a warp per row
-                const int c = lane & 15;
-                uint8_t* qs = smem + blk * AS_TILE + (c >> 3) * (AS_TILE / 2);
-                uint4 v[16];
-                const int row0 = warp * 32 + (lane >> 4);
-                int q = (x.r0 + row0) / G, g = x.r0 + row0 - q * G;
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(x.row_base + q) * a.nq + x.kvh * G + g) * 128) + c;
-                const size_t step = (size_t)(a.nq - G) * 16;        // from the last head of a row to the first of the next
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (row0 + 2 * i < x.n_valid) v[i] = __ldg(src);
-                    #pragma unroll
-                    for (int k = 0; k < 2; ++k) { src += 16; if (++g == G) { g = 0; src += step; } }
-                }
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int row = (warp & 3) * 32 + 2 * i + (lane >> 4);
-                    *reinterpret_cast<uint4*>(qs + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[i];
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[blk]);
-            }
             int lo = 0, hi = 0;
             if (tid < x.n_valid) {
                 if (p.prefixes) hi = x.cached;
@@ -463,10 +452,12 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                 auto chunk_at = [&](int c, float (&v)[32]) { tc_ld32(ts + c * 32, v); };
                 const bool clear = !gone && kb + AS_TK <= x.all_hi && (kb >= x.all_lo || kb + AS_TK <= x.sinks);
                 auto mask = [&](int c, float (&v)[32]) {
-                    if (!clear) {
-                        const int nh = (gone ? 0 : hi - kb) - c * 32, nl = lo - kb - c * 32, ns = x.sinks - kb - c * 32;
+                    if (!clear) {                            // keys that the row sees, as bits: a predicate per key and no comparisons
+                        auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+                        const int k0 = kb + c * 32;
+                        const uint32_t see = gone ? 0u : below(hi - k0) & (~below(lo - k0) | below(x.sinks - k0));
                         #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = i < nh && (i >= nl || i < ns) ? v[i] : -INFINITY;
+                        for (int i = 0; i < 32; ++i) v[i] = see >> i & 1 ? v[i] : -INFINITY;
                     }
                 };
                 float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -567,8 +558,16 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             const int sr = lane >> 2, sc = lane & 3;
             // 32 columns of the warp's rows in fp16, or 16 in fp32, by way of shared memory: rows of 64 bytes, eight per instruction
             size_t at[4];                                                   // of rows sr, 8 + sr, ..
-            #pragma unroll
-            for (int g = 0; g < 4; ++g) at[g] = row_of(min(8 * g + sr, max(n_mine - 1, 0)));
+            {
+                const int pk = x.r0 + warp * 32 + sr;
+                int q = pk / G, g0 = pk - q * G;
+                #pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    at[g] = (size_t)(x.row_base + q) * a.nq + x.kvh * G + g0;
+                    q += per8; g0 += left8;
+                    if (g0 >= G) { g0 -= G; ++q; }
+                }
+            }
             auto put = [&](const uint4 (&v)[4], auto store) {
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = v[i];

@@ -162,7 +162,7 @@ WINDOWS = [
     ([5], [300], 1, 0, 40, 8), ([5], [300], 1, 3, 40, 8), ([3], [100], 64, 60, 16, 8), ([3], [100], 64, 500, 16, 8), ([40], [0], 16, 4, 16, 8),
     # head ratios: none shared, odd, more than a row block
     ([1, 3], [500, 77], 200, 4, 6, 6), ([1, 2, 9], [500, 1000, 3], 333, 5, 9, 3), ([2, 1], [70, 900], 128, 4, 32, 1), ([7, 30], [600, 20], 100, 9, 28, 4),
-    ([1], [400], 100, 2, 192, 1),
+    ([1], [400], 100, 2, 128, 1), ([3, 1], [400, 90], 100, 2, 100, 1), ([40, 1, 2], [300, 90, 1000], 333, 2, 17, 1), ([90], [300], 333, 2, 33, 1),
     # ragged: sequences without rows, decode rows beside chunks, many short ones, one after a long window
     ([0, 1, 0, 130, 1, 0], [10, 2000, 0, 513, 0, 99], 512, 4, 40, 8), ([1] * 40, list(range(0, 4000, 100)), 1024, 4, 16, 8),
     ([1, 64, 1, 2, 333], [3000, 100, 5, 1500, 1], 256, 70, 32, 4), ([1, 1], [9000, 5], 8192, 300, 40, 8), ([300], [1000], 5000, 0, 16, 2),
@@ -426,7 +426,7 @@ BAD = [(dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(bt=0), -1), (dic
        (dict(k=4100), -1), (dict(v=4100), -1), (dict(bsz=-1), -1), (dict(q_len=-1), -1), (dict(rows=3), -1), (dict(rows=-1), -1), (dict(nq=0), -1),
        (dict(nkv=0), -1), (dict(nq=12), -1), (dict(hd=64), -2), (dict(pages=0), -1), (dict(pps=0), -1), (dict(pps=1 << 23), -1), (dict(scale=-1.0), -1),
        (dict(scale=math.nan), -1), (dict(scale=math.inf), -1), (dict(bsz=1 << 30, rows=1 << 30), -2), (dict(bsz=8193, rows=8193), -2),
-       (dict(nq=1 << 20, rows=1 << 11, cu=4096), -1)]
+       (dict(nq=8 * 128, rows=1 << 21, cu=4096), -1), (dict(nq=8 * 129), -2)]
 BAD_WINDOW = [(dict(window=0), -1), (dict(window=-3), -1), (dict(sinks=-1), -1)]
 BAD_PREFIX = [(dict(groups=-1), -1), (dict(groups=3), -1), (dict(gs=0), -1), (dict(pl=0), -1)]
 
