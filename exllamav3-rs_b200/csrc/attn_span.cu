@@ -25,6 +25,12 @@ int span_check(exl3_ctx* ctx, const SpanArgs& a, int hd, float sm_scale, const c
     if (a.bsz > 32 * AS_MAX_CHUNKS) return bad(EXL3_ERR_UNSUPPORTED, "more than 8192 sequences");
     if ((long long)a.rows * a.nq > 1LL << 30) return bad(EXL3_ERR_INVALID, "too many rows");
     if (hd != 128) return bad(EXL3_ERR_UNSUPPORTED, "head_dim must be 128");
+    // The kernels count key tiles in 32 bits: of 16 keys over the sequences of a launch, of 128 keys over a head's row blocks (a block has more
+    // than half of its rows)
+    const double keys = std::min((double)a.pps * EXL3_PAGE, (double)a.window + a.sinks + a.q_len) + 512;
+    const double blocks = (double)a.rows * (a.nq / a.nkv) / (AS_BLOCK / 2) + a.bsz;
+    if (std::min(a.bsz, AR_MAX_BSZ) * keys / 16 >= 2147483648.0 || blocks * keys / AS_TK >= 2147483648.0)
+        return bad(EXL3_ERR_UNSUPPORTED, "rows and block tables of more than 2^31 key tiles");
     if (!span_empty(a) && (!a.q || !a.o || !a.kc || !a.vc || !a.block_table || !a.seqlens)) return bad(EXL3_ERR_INVALID, "null argument");
     if (!aligned16(a.q) || !aligned16(a.o) || !aligned16(a.kc) || !aligned16(a.vc)) return bad(EXL3_ERR_INVALID, "pointers must be 16-byte aligned");
     if (!(sm_scale >= 0.f) || isinf(sm_scale)) return bad(EXL3_ERR_INVALID, "sm_scale must be finite and not negative");
@@ -166,7 +172,7 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     // A few sequences of few rows read a short prefix sooner each than together, which is two kernels more: up to 128 MB read again (as far as the
     // host knows, from the table's width).  us, each and together, 16 / 8 heads, sequences x prefix: 4 x 512 18 and 30, 8 x 2048 24 and 32,
     // 16 x 2048 36 and 39, 32 x 1024 37 and 34; 40 / 8 heads: 4 x 8192 41 and 44, 8 x 8192 59 and 46.
-    const bool alone = a.n_groups > 0 && !any_long && (long long)(a.bsz - 1) * a.pps * EXL3_PAGE * a.nkv * 512 <= 128LL << 20;
+    const bool alone = a.n_groups > 0 && !any_long && (double)(a.bsz - 1) * a.pps * EXL3_PAGE * a.nkv * 512 <= 128.0 * (1 << 20);
     const bool groups = a.n_groups > 0 && !alone;
     // Two row blocks share the tiles where a group or a sequence may have that many rows
     const bool two_prefix = all > (long long)AS_BLOCK * a.n_groups, two_own = packed > AS_BLOCK;
@@ -192,7 +198,7 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     }
     exl3_chain_scope chain(ctx, groups);
     // Both classes of a batch over windows, where neither is small beside the other: each gets its share of the SMs, and the start and end of
-    // one kernel, 10 us and more, runs under the other (28 rows beside 4 x 251, window 1024: 104 us one after the other).
+    // one kernel, 10 us and more, runs under the other (28 rows beside 4 x 251, window 1024: 89 us, one after the other 104).
     const int aside = any_long && any_few && !groups && a.n_groups == 0 ? span_aside(ctx, a) : 0;
     if (aside) {
         if (cudaEventRecord(ctx->ev_fork, st) != cudaSuccess || cudaStreamWaitEvent(ctx->aux_stream, ctx->ev_fork, 0) != cudaSuccess)
@@ -225,6 +231,7 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     if (groups) {
         const SpanJoinParams j = {a, prefix, share, p.rest};
         const long long pairs = (long long)a.rows * a.nq;
+        // us, whole calls, one pair per warp and four: 64 x 16 pairs 69 and 74, 1024 x 40 pairs 884 and 846
         if (pairs <= 64LL * ctx->num_sms) exl3_launch(ctx, span_join_kernel<1>, (unsigned)((pairs + 7) / 8), 256, 0, st, j);
         else exl3_launch(ctx, span_join_kernel<4>, (unsigned)((pairs + 31) / 32), 256, 0, st, j);
         ctx->launches++;

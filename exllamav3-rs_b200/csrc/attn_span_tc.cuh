@@ -10,7 +10,12 @@
 // chain of scores, softmax, product that a block cannot overlap with itself.  So an SM holds two blocks, whose softmax runs under the
 // other's products: NB = 2, one CTA whose blocks share every tile, where sequences have the rows (with two CTAs that read tiles of their own
 // 4 x 2048 rows took 794 us: 64 KB per 2500 cycles and SM is what L2 gives); NB = 1, two CTAs of one block, where they do not, so that
-// the start and end of short units overlap.
+// the start and end of short units overlap.  4 x 2048 rows over windows of 4096: 712 us, 845 TFLOP/s; 8 x 128 rows over 8192 shared keys and 512 to
+// 2000 of their own: 846 us, 815 TFLOP/s.  (A quarter or a sixth of the exponentials by a polynomial instead: 728 and 720 for 725 us, so
+// they are not what a tile waits for; P announced after 96 keys instead of 64: 710 and 893 for 712 and 846 us.)
+//
+// Queries come as copies of whole rows, a unit ahead: a unit has rows * G <= 128 NB packed rows (read by the softmax threads at a unit's
+// start instead: 4 x 2048 rows 779 us).
 //
 // The tiles of all units stand in one line, of which every CTA takes an equal part (one item per CTA, with the splits chosen for the fewest
 // waves, left SMs idle for 30 % of 8 x 128 rows over 8192 shared keys: 160 units on 148 SMs).  The parts are found from the lengths by each
@@ -160,26 +165,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
     asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
     return o;
 }
-
-// 2^x of two values without the special-function unit: x to the nearest integer by adding 1.5 * 2^23, a polynomial of degree 5 for what is
-// left in [-1/2, 1/2] (relative error 7.5e-8; coefficients by the Remez exchange for the relative error), the integer added to the
-// exponent.  Values below -126, minus infinity among them, count as -126.
-__device__ __forceinline__ float2 exp2_poly(float2 x)
-{
-    auto both = [](float v) { return make_float2(v, v); };
-    x.x = fmaxf(x.x, -126.f); x.y = fmaxf(x.y, -126.f);
-    const float2 r = add2(x, both(12582912.f));
-    const float2 f = fma2(add2(r, both(-12582912.f)), both(-1.f), x);
-    float2 y = fma2(f, both(0.0013276472454890609f), both(0.009675540961325169f));
-    y = fma2(y, f, both(0.05550713092088699f));
-    y = fma2(y, f, both(0.24022120237350464f));
-    y = fma2(y, f, both(0.6931469440460205f));
-    y = fma2(y, f, both(1.0000001192092896f));
-    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23)));
-}
-#ifndef AS_POLY
-#define AS_POLY 4
-#endif
 
 template <int NB>
 __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -510,7 +495,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                     #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 y = fma2(make_float2(v[i], v[i + 1]), scale2, nref2);
-                        const float2 ex = (i >> 1) % AS_POLY == AS_POLY - 1 ? exp2_poly(y) : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                        const float2 ex = make_float2(ex2_approx(y.x), ex2_approx(y.y));
                         sum = add2(sum, ex);
                         w[at + (i >> 1)] = pack_h2(ex.x, ex.y);             // the one rounding of a weight, as the product takes it
                     }

@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(RP_THREADS, 4) rope_paged_kernel(const RopePag
 {
     pdl_enter_first(early);
     // cos, sin of a row's frequencies, times attn_factor, as the lanes read them: pairs of frequencies, the pairs of all lanes side by side
-    // (frequency after frequency, a lane's 64 bytes apart, the reads' bank conflicts were what 8192 rows waited for: 68 us)
+    // (frequency after frequency, a lane's 64 bytes apart, the reads' bank conflicts were what 8192 rows waited for: 68 us, and 51 without)
     __shared__ __align__(16) float4 s_cs[R][32];
     __shared__ int s_pos[R];                                    // place in the sequence; -1: the row belongs to none
     __shared__ long long s_slot[R];                             // token slot in the pools; -1: none

@@ -232,7 +232,12 @@ EXL3_API int exl3_rope_append_paged(exl3_ctx* ctx, exl3_stream stream, const exl
  * j < sinks (window >= 1, sinks >= 0).  The call's own keys are in the pools already (exl3_rope_append_paged,
  * exl3_paged_kv_cache_update).  Block-table entries none of whose keys is visible are not read, so pages behind the window can be
  * released (and their entries be -1); the keys of an entry outside the pool are left out.  A row that sees nothing gives zeros.  sm_scale
- * 0 = 1/sqrt(hd), negative ones are refused. */
+ * 0 = 1/sqrt(hd), negative ones are refused.
+ * What no row of a sequence sees may hold anything; a value that is not finite at a key that some of a sequence's (or group's) rows see can
+ * reach those that do not.  o must not overlap q or the pools.  Limits, EXL3_ERR_UNSUPPORTED beyond: 128 query heads per kv head, 8192
+ * sequences, 2^31 key tiles by the rows' and tables' sizes; rows * nq <= 2^30.  Partial sums go to the context's scratch: 10 MB for
+ * sequences of up to 16 rows (query heads of a kv head times tokens), 40 MB for longer ones, of the size it was created with;
+ * EXL3_ERR_WORKSPACE where it is too small. */
 EXL3_API int exl3_window_attn_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, const void* k_cache, const void* v_cache,
                            const int32_t* block_table, const int32_t* cache_seqlens, const int32_t* cu_q, void* o, int bsz, int q_len,
                            int rows, int nq, int nkv, int hd, int pages, int pages_per_seq, int window, int sinks, float sm_scale);
@@ -241,7 +246,9 @@ EXL3_API int exl3_window_attn_paged(exl3_ctx* ctx, exl3_stream stream, const voi
  * (int32 [n_groups+1], device, ascending), whose first prefix_lens[g] tokens (int32 [n_groups], device) are the same - the same pages,
  * as exl3_pool_alloc_prefix gives them, or copies - and are read once for the whole group, through the block table of its first sequence.
  * The keys behind them, and all keys of sequences in no group, are read through a sequence's own table.  A sequence that has cached less
- * than the prefix is computed on its own.  Otherwise as above. */
+ * than the prefix is computed on its own.  A group's first table has to hold the prefix also where that sequence has no rows, or has cached
+ * less.  Otherwise as above; scratch: rows * nq * 528 bytes twice over at least (and up to a quarter of the scratch, for prefixes split among
+ * more SMs) beside the window's. */
 EXL3_API int exl3_prefix_attn_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, const void* k_cache, const void* v_cache,
                            const int32_t* block_table, const int32_t* cache_seqlens, const int32_t* cu_q, const int32_t* group_start,
                            const int32_t* prefix_lens, int n_groups, void* o, int bsz, int q_len, int rows, int nq, int nkv, int hd,

@@ -427,6 +427,8 @@ BAD = [(dict(q=0), -1), (dict(k=0), -1), (dict(v=0), -1), (dict(bt=0), -1), (dic
        (dict(nkv=0), -1), (dict(nq=12), -1), (dict(hd=64), -2), (dict(pages=0), -1), (dict(pps=0), -1), (dict(pps=1 << 23), -1), (dict(scale=-1.0), -1),
        (dict(scale=math.nan), -1), (dict(scale=math.inf), -1), (dict(bsz=1 << 30, rows=1 << 30), -2), (dict(bsz=8193, rows=8193), -2),
        (dict(nq=8 * 128, rows=1 << 21, cu=4096), -1), (dict(nq=8 * 129), -2)]
+WIDE = [(dict(bsz=1024, rows=1024, pps=1 << 17, window=1 << 30), -2),
+        (dict(rows=1 << 24, q_len=1 << 24, cu=4096, nq=64, nkv=8, pps=1 << 12, window=1 << 30), -2)]     # 2^31 key tiles and more
 BAD_WINDOW = [(dict(window=0), -1), (dict(window=-3), -1), (dict(sinks=-1), -1)]
 BAD_PREFIX = [(dict(groups=-1), -1), (dict(groups=3), -1), (dict(gs=0), -1), (dict(pl=0), -1)]
 
@@ -447,7 +449,7 @@ def test_refusals_on_the_host(which):
     assert _call(lib, which, None) == -1
     fake = C.create_string_buffer(1 << 16)
     C.memset(fake, 0xff, 4)                                # a device that never is the current one
-    for change, code in BAD + (BAD_WINDOW if which == "window" else BAD_PREFIX):
+    for change, code in BAD + WIDE + (BAD_WINDOW if which == "window" else BAD_PREFIX):
         assert _call(lib, which, fake, **change) == code, change
     assert _call(lib, which, fake) == -1 and b"device" in lib.exl3_last_error(fake)
 
