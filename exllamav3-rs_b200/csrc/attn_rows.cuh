@@ -62,7 +62,6 @@ struct ArParams {
     int* counters;                                      // [CTAs][4], zero between calls
     int* status;
     float* rest;                                        // [rows][nq][AR_MS] partial sums of sequences that a prefix is added to
-    int alone;                                          // prefixes are read here too, through their own table, by each sequence
     int first;                                          // nothing of this call is in front of the launch
 };
 
@@ -72,7 +71,9 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
                  ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)) : "memory");
 }
 
-template <int HW>
+// ALONE: prefixes are read here too, through their own table, by each sequence.  (A kernel of its own: with both kinds of tiles in every loop
+// 128 rows over windows of 4096 took 210 us for 193, a row over 1024 13.4 for 12.6.)
+template <int HW, bool ALONE>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_constant__ ArMaps maps, const ArParams p, int early)
 {
     using Cfg = ArCfg<HW>;
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
         if (s.ql == 0 || s.ql * G > AR_ROWS) return 0;
         const int len = span_group(a, b, s.cached).len;
         const SpanTiles t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, len);
-        return max((p.alone ? (len + TK - 1) / TK : 0) + t.sink + t.near, 1);
+        return max((ALONE ? (len + TK - 1) / TK : 0) + t.sink + t.near, 1);
     };
     for (int b = tid; b < p.bsz; b += AR_THREADS) sum[b] = tiles_of(p.b0 + b);
     __syncthreads();
@@ -178,17 +179,17 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                 s = span_seq(a, gb);
                 grp = span_group(a, gb, s.cached);
                 t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, grp.len);
-                n_pre = p.alone ? (grp.len + TK - 1) / TK : 0;
+                n_pre = ALONE ? (grp.len + TK - 1) / TK : 0;
                 have = b;
             }
             page0 = -64;
             const long long u0 = f - from;
             for (int i = from; i < upto; ++i, ++it) {
                 const int stage = it % AR_STAGES;
-                const bool pre = i < n_pre;
+                const bool pre = ALONE && i < n_pre;
                 const int own = i - n_pre, kt = pre ? i : t.sink + t.near == 0 ? -1 : own < t.sink ? own : t.first + (own - t.sink);
                 const int32_t* bt = a.block_table + (size_t)(pre ? grp.first : gb) * a.pps;
-                if (i == n_pre) page0 = -64;
+                if (ALONE && i == n_pre) page0 = -64;
                 int page = -1;
                 if (kt >= 0) {
                     const int pg = kt / PER_PAGE;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                     if (cut) { units[n_unit % AR_UNITS].c0 = c0; units[n_unit % AR_UNITS].pieces = c1 - c0 + 1; }
                     if (i == from) {
                         ArUnit& u = units[n_unit % AR_UNITS];
-                        u.b = gb; u.hg = hg; u.row_base = s.row_base; u.ql = s.ql; u.cached = s.cached; u.key_lo = grp.len; u.group = p.alone ? -1 : grp.g;
+                        u.b = gb; u.hg = hg; u.row_base = s.row_base; u.ql = s.ql; u.cached = s.cached; u.key_lo = grp.len; u.group = ALONE ? -1 : grp.g;
                         u.whole = from == 0 && upto == n;
                         u.slot = 2 * c + (from == 0 ? 1 : 0);
                         u.tiles = upto - from;
@@ -298,8 +299,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
             if (i > 0 && !mbar_wait_warp(&full[st0], (it / AR_STAGES) & 1)) { ok = false; break; }
             if (two && !mbar_wait_warp(&full[st1], ((it + 1) / AR_STAGES) & 1)) { ok = false; break; }
             const int kt0 = tile_of[st0], kt1 = two ? tile_of[st1] : -1;
-            const bool pre0 = kt0 >= AR_PREFIX, pre1 = kt1 >= AR_PREFIX;             // of a prefix: every row sees all of it
-            const int kb0 = (kt0 & (AR_PREFIX - 1)) * TK + wk * 16, kb1 = (kt1 & (AR_PREFIX - 1)) * TK + wk * 16;     // first key of this warp's in either
+            const bool pre0 = ALONE && kt0 >= AR_PREFIX, pre1 = ALONE && kt1 >= AR_PREFIX;             // of a prefix: every row sees all of it
+            const int kb0 = (ALONE ? kt0 & (AR_PREFIX - 1) : kt0) * TK + wk * 16, kb1 = (ALONE ? kt1 & (AR_PREFIX - 1) : kt1) * TK + wk * 16;     // first key of this warp's in either
             auto seen = [&](int kt, int kb, bool pre) { return kt >= 0 && (pre ? kb < u.key_lo : kb < any_hi && (kb + 16 > any_lo || kb < a.sinks)); };
             auto whole = [&](int kt, int kb, bool pre) { return kt >= 0 && (pre ? kb + 16 <= u.key_lo : kb + 16 <= all_hi && (kb >= all_lo || kb + 16 <= a.sinks)); };
             const bool in0 = seen(kt0, kb0, pre0), in1 = seen(kt1, kb1, pre1);

@@ -100,8 +100,8 @@ constexpr size_t AR_SCRATCH = (size_t)AR_WARPS * AR_ROWS * AR_MS * 4;       // p
 // Keys that a CTA takes at least: fewer are more partial sums to join (us at 64, 128 and 192 keys: one row over a window of 1024 16.2, 15.5 and
 // 20.7, of 4096 26, 20 and 23)
 constexpr int AR_MIN_KEYS = 128;
-template <int HW>
-int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool alone, bool plain, const AsParams& pre, int sms, size_t* ws_off)
+template <int HW, bool ALONE>
+int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool plain, const AsParams& pre, int sms, size_t* ws_off)
 {
     using Cfg = ArCfg<HW>;
     ArMaps maps;
@@ -110,7 +110,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     if (Cfg::KW == 1) { maps.k16 = maps.k; maps.v16 = maps.v; }
     static bool done[64] = {};
-    if (!span_configure(attn_rows_kernel<HW>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    if (!span_configure(attn_rows_kernel<HW, ALONE>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int ctas = sms;
     ArParams p;
     p.a = a;
@@ -118,7 +118,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
     p.partial = (float*)exl3_ws_take(ctx, ws_off, 2 * ctas * AR_SCRATCH);
     if (!p.partial) return exl3_fail(ctx, EXL3_ERR_WORKSPACE, "attention: context scratch too small for the partial sums");
     p.counters = ctx->counters; p.status = ctx->status;
-    p.rest = pre.rest; p.alone = alone;
+    p.rest = pre.rest;
     for (int b0 = 0; b0 < a.bsz; b0 += AR_MAX_BSZ) {
         p.b0 = b0; p.bsz = std::min(AR_MAX_BSZ, a.bsz - b0);
         p.first = first || b0 > 0;                          // launches of one call share the partial sums
@@ -126,8 +126,8 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
                                         ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1) + 1;
         const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
-        if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
-        else exl3_launch(ctx, attn_rows_kernel<HW>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
+        if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
+        else exl3_launch(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
         ctx->launches++;
     }
     return EXL3_OK;
@@ -205,8 +205,8 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
             return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream fork failed");
         const int chained = ctx->chain;
         ctx->chain = 0;                                      // a plain launch: nothing of the second stream is in front
-        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, ctx->aux_stream, a, true, false, true, p, aside, &off)
-                            : span_rows<1>(ctx, ctx->aux_stream, a, true, false, true, p, aside, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4, false>(ctx, ctx->aux_stream, a, true, true, p, aside, &off)
+                            : span_rows<1, false>(ctx, ctx->aux_stream, a, true, true, p, aside, &off);
         ctx->chain = chained;
         ctx->chain_break = 1;
     }
@@ -224,8 +224,9 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     if (rc) return rc;
     exl3_chain_scope behind(ctx, any_long);
     if (any_few) {
-        rc = a.nkv % 4 == 0 ? span_rows<4>(ctx, st, a, p.first != 0, alone, false, p, ctx->num_sms, &off)
-                            : span_rows<1>(ctx, st, a, p.first != 0, alone, false, p, ctx->num_sms, &off);
+        const bool four = a.nkv % 4 == 0, first = p.first != 0;
+        rc = alone ? four ? span_rows<4, true>(ctx, st, a, first, false, p, ctx->num_sms, &off) : span_rows<1, true>(ctx, st, a, first, false, p, ctx->num_sms, &off)
+                   : four ? span_rows<4, false>(ctx, st, a, first, false, p, ctx->num_sms, &off) : span_rows<1, false>(ctx, st, a, first, false, p, ctx->num_sms, &off);
         if (rc) return rc;
     }
     if (groups) {
