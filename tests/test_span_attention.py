@@ -397,6 +397,32 @@ def test_two_contexts_on_two_streams(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,mb", [(32, 90), (25, 84), (12, 72)])
+def test_prefix_with_little_scratch(rows, mb):
+    """partial sums of 20 sequences' prefixes: a place per row and head has room once (prefixes stay whole), twice, and three times"""
+    import exl3b200
+    place = 20 * rows * 40 * 528
+    assert (mb << 18) // place == {32: 1, 25: 2, 12: 3}[rows]
+    small = exl3b200.Ctx(0, workspace_bytes=mb << 20)
+    b = Batch([rows] * 20, [2000 + 30 * i for i in range(20)], 40, 8, groups=[0, 11, 20], prefix=[1900, 1000], seed=21)
+    b.check(prefix(small, b))
+    small.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens", [[1, 1], [40, 1]])
+def test_too_little_scratch_is_refused(q_lens):
+    import exl3b200
+    small = exl3b200.Ctx(0, workspace_bytes=1 << 20)
+    b = Batch(q_lens, [100, 300], 16, 8, 64, 4, groups=[0, 2], prefix=[64], seed=22)
+    for call in (window, prefix):
+        with pytest.raises(exl3b200.Exl3Error, match="scratch"):
+            call(small, b)
+    assert bool((b.o == 7.0).all())
+    small.close()
+
+
+@pytest.mark.gpu
 def test_empty_calls(ctx):
     import torch
     f = lambda *s: torch.zeros(s, dtype=torch.float16, device="cuda")  # noqa: E731
