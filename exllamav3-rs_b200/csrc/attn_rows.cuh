@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
                 for (int nb = 0; nb < 4; ++nb)
                     #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = s[nb][e] * a.scale_log2;
+                        float v = __fmul_rn(s[nb][e], a.scale_log2);      // rounded here as in the maximum: not fused with the subtraction below
                         if (!clear) {
                             const int key = (nb < 2 ? kb0 : kb1) + (nb & 1) * 8 + 2 * t4 + (e & 1), h = e >> 1;
                             const bool in = nb < 2 ? in0 : in1, pre = nb < 2 ? pre0 : pre1;

@@ -32,6 +32,10 @@ constexpr int AS_BLOCK = 128;                            // rows of a block: the
 constexpr int AS_TILE = AS_TK * 256;                    // bytes of a tile of K, V or Q: two 64-dim halves of 16 KB
 constexpr int AS_MAX_SPLITS = 32;
 constexpr int AS_MAX_CHUNKS = 256;                      // of 32 sequences
+// An exponent is one fused score * scale - reference, whose product is not rounded, against a reference that is: off by half a step of the
+// reference, for all keys of a part of a row alike but not for its other parts, and from 2^28 on by more than fp16 weights hold (they came out
+// infinite, the output NaN).  Where a reference is this far from 0, where half a step is 2^-12, the maximum is subtracted ahead of the scale.
+constexpr float AS_FAR = 8192.0f;
 
 // A unit's part in work, as the producer finds it
 struct AsPiece {
@@ -424,7 +428,9 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
             auto key_tile = [&](int j) -> int { const int i = x.t0 + j; return i < x.sink ? i : x.first + (i - x.sink); };
             // a tile's page is read a tile ahead and looked at where it counts: a comparison behind the load waits for it (860 cycles per tile)
             int page = x.any ? bt[key_tile(0) >> 1] : -1;
-            float m_used = -INFINITY, m_true = -INFINITY, l = 0.f;
+            // m_used: the exponents' reference; r_true: the maximum before the scale, which is positive
+            float m_used = -INFINITY, r_true = -INFINITY, l = 0.f;
+            bool far = false;                                               // of the warp, from some tile on
             for (int j = 0; j < x.n_tiles; ++j, ++done) {
                 const int kb = key_tile(j) * AS_TK;
                 const bool gone = page < 0 || page >= a.pages;
@@ -450,21 +456,28 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                     #pragma unroll
                     for (int i = 0; i < 32; i += 4) { mx0 = fmax3(mx0, v[i], v[i + 1]); mx1 = fmax3(mx1, v[i + 2], v[i + 3]); }
                 };
-                chunk_at(2, x0); chunk_at(3, x1); chunk_at(0, x2);
-                tc_wait_ld();
-                mask(2, x0); maximum(x0);
-                chunk_at(1, x0);
-                mask(3, x1); maximum(x1);
-                mask(0, x2); maximum(x2);
-                tc_wait_ld();
-                mask(1, x0); maximum(x0);
-                m_true = fmaxf(m_true, fmaxf(mx0, mx1) * scale);            // raw scores: the scale is positive
-                // the reference of the exponents moves only when the maximum has grown by 2^8, so O is seldom rescaled
-                const bool move = m_true > m_used + ATC_RESCALE_THRESHOLD || (m_used == -INFINITY && m_true > -INFINITY);
-                const bool rescale = move && m_used != -INFINITY;
-                const float corr = rescale ? ex2_approx(m_used - m_true) : 1.0f;
-                if (move) m_used = m_true;
-                if (__any_sync(0xffffffffu, rescale)) {                     // O holds the tiles before: the scores came after their product
+                // values that no row of the unit sees may be anything (0 * NaN would spoil O): cleared by the first block, whose product
+                // comes first, a key per thread
+                auto clear_values = [&]() -> bool {
+                    if (blk != 0 || gone || (kb + AS_TK <= x.end && (kb >= x.lo || kb + AS_TK <= x.sinks))) return true;
+                    const int item = x.ring + 2 * j + 1, slot = item % SLOTS;
+                    if (!mbar_wait_sleep_warp(&kv_full[slot], (item / SLOTS) & 1)) return false;
+                    const int key = kb + r;
+                    if (!(key < x.end && (key >= x.lo || key < x.sinks))) {
+                        #pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            *reinterpret_cast<uint4*>(smem + Cfg::OFF_KV + slot * AS_TILE + (c >> 3) * (AS_TILE / 2) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                    return true;
+                };
+                auto announce = [&](uint64_t* bar) {
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                auto rescale_o = [&](float corr) {                          // O holds the tiles before: the scores came after their product
                     #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         tc_ld32(to_ + c * 32, x1);
@@ -473,53 +486,95 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
                         for (int i = 0; i < 32; ++i) x1[i] *= corr;
                         tc_st32(to_ + c * 32, x1);
                     }
-                }
-                // values that no row of the unit sees may be anything (0 * NaN would spoil O): cleared by the first block, whose product
-                // comes first, a key per thread
-                if (blk == 0 && !gone && !(kb + AS_TK <= x.end && (kb >= x.lo || kb + AS_TK <= x.sinks))) {
-                    const int item = x.ring + 2 * j + 1, slot = item % SLOTS;
-                    if (!mbar_wait_sleep_warp(&kv_full[slot], (item / SLOTS) & 1)) { failed = true; break; }
-                    const int key = kb + r;
-                    if (!(key < x.end && (key >= x.lo || key < x.sinks))) {
-                        #pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            *reinterpret_cast<uint4*>(smem + Cfg::OFF_KV + slot * AS_TILE + (c >> 3) * (AS_TILE / 2) + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();
-                }
-                const float nref = m_used == -INFINITY ? 0.f : -m_used;
-                const float2 scale2 = make_float2(scale, scale), nref2 = make_float2(nref, nref);
+                };
                 float2 sum = make_float2(0.f, 0.f);
-                uint32_t w[32];
-                auto weights = [&](const float (&v)[32], int at) {
+                const bool entered = !far;
+                if (!far) {
+                    chunk_at(2, x0); chunk_at(3, x1); chunk_at(0, x2);
+                    tc_wait_ld();
+                    mask(2, x0); maximum(x0);
+                    chunk_at(1, x0);
+                    mask(3, x1); maximum(x1);
+                    mask(0, x2); maximum(x2);
+                    tc_wait_ld();
+                    mask(1, x0); maximum(x0);
+                    r_true = fmaxf(r_true, fmaxf(mx0, mx1));
+                    const float m_true = __fmul_rn(r_true, scale);
+                    // the reference moves only when the maximum has grown by 2^8, so O is seldom rescaled
+                    const bool move = m_true > m_used + ATC_RESCALE_THRESHOLD || (m_used == -INFINITY && m_true > -INFINITY);
+                    float corr = 1.0f;
+                    if (__any_sync(0xffffffffu, move)) {
+                        far = __any_sync(0xffffffffu, move && hi > 0 && fabsf(m_true) >= AS_FAR);     // rows behind the unit's last may hold anything
+                        if (!far) {
+                            const bool rescale = move && m_used != -INFINITY;
+                            if (rescale) corr = ex2_approx(m_used - m_true);
+                            if (move) m_used = m_true;
+                            if (__any_sync(0xffffffffu, rescale)) rescale_o(corr);
+                        }
+                    }
+                    if (!far) {
+                        if (!clear_values()) { failed = true; break; }
+                        const float nref = m_used == -INFINITY ? 0.f : -m_used;
+                        const float2 scale2 = make_float2(scale, scale), nref2 = make_float2(nref, nref);
+                        uint32_t w[32];
+                        auto weights = [&](const float (&v)[32], int at) {
+                            #pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 y = fma2(make_float2(v[i], v[i + 1]), scale2, nref2);
+                                const float2 ex = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                                sum = add2(sum, ex);
+                                w[at + (i >> 1)] = pack_h2(ex.x, ex.y);             // the one rounding of a weight, as the product takes it
+                            }
+                        };
+                        chunk_at(2, x1);
+                        weights(x2, 0);
+                        weights(x0, 16);
+                        tc_st32u(ts, w);
+                        tc_wait_ld();
+                        announce(&p_half[blk]);
+                        chunk_at(3, x0);
+                        mask(2, x1);
+                        weights(x1, 0);
+                        tc_wait_ld();
+                        mask(3, x0);
+                        weights(x0, 16);
+                        tc_st32u(ts + 32, w);
+                        announce(&p_full[blk]);
+                        l = l * corr + (sum.x + sum.y);
+                        continue;
+                    }
+                }
+                // A reference far from 0, in this tile or one before: 32 scores at a time, and the reference is always the maximum.  (A way of its own to
+                // the end of the tile; within the other one it took 2 % more of every call.)
+                const float r_before = r_true;
+                #pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    chunk_at(c, x0);
+                    tc_wait_ld();
+                    mask(c, x0);
+                    maximum(x0);
+                }
+                r_true = fmaxf(r_true, fmaxf(mx0, mx1));
+                const float m_true = __fmul_rn(r_true, scale), grown = entered ? m_used - m_true : (r_before - r_true) * scale;
+                const float corr = m_used != -INFINITY && grown < 0.f ? ex2_approx(grown) : 1.0f, origin = r_true == -INFINITY ? 0.f : r_true;
+                m_used = m_true;
+                if (__any_sync(0xffffffffu, corr != 1.0f)) rescale_o(corr);
+                if (!clear_values()) { failed = true; break; }
+                #pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    chunk_at(c, x0);
+                    tc_wait_ld();
+                    mask(c, x0);
+                    uint32_t w[16];
                     #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float2 y = fma2(make_float2(v[i], v[i + 1]), scale2, nref2);
-                        const float2 ex = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                        const float2 ex = make_float2(ex2_approx((x0[i] - origin) * scale), ex2_approx((x0[i + 1] - origin) * scale));
                         sum = add2(sum, ex);
-                        w[at + (i >> 1)] = pack_h2(ex.x, ex.y);             // the one rounding of a weight, as the product takes it
+                        w[i >> 1] = pack_h2(ex.x, ex.y);
                     }
-                };
-                auto announce = [&](uint64_t* bar) {
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar);
-                };
-                chunk_at(2, x1);
-                weights(x2, 0);
-                weights(x0, 16);
-                tc_st32u(ts, w);
-                tc_wait_ld();
-                announce(&p_half[blk]);
-                chunk_at(3, x0);
-                mask(2, x1);
-                weights(x1, 0);
-                tc_wait_ld();
-                mask(3, x0);
-                weights(x0, 16);
-                tc_st32u(ts + 32, w);
-                announce(&p_full[blk]);
+                    tc_st16u(ts + c * 16, w);                               // over scores that are read already
+                    if (c & 1) announce(c == 1 ? &p_half[blk] : &p_full[blk]);
+                }
                 l = l * corr + (sum.x + sum.y);
             }
             failed = __any_sync(0xffffffffu, failed);

@@ -509,3 +509,78 @@ def test_wrapper_checks_shapes(ctx):
     for gs, pl in ((i(2), i(2)), (i(4), i(3))):
         with pytest.raises(exl3b200.Exl3Error):
             ctx.prefix_attn_paged(**good, group_start=gs, prefix_lens=pl)
+
+
+# --------------------------------------------------------------------------------------------------------- scores far from 0
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dims", [1, 128])
+@pytest.mark.parametrize("size", [2.0 ** 6, 2.0 ** 9, 2.0 ** 12, 2.0 ** 14])
+@pytest.mark.parametrize("q_lens,groups", [([1, 1], None), ([60, 1], None), ([130], None), ([1] * 4, [0, 4]), ([1, 40], [0, 2])])
+def test_scores_of_any_size(ctx, q_lens, groups, size, dims):
+    """Every third key has the largest score, the others 0: the output is the mean of the former's values.  All products and sums are exact in
+    fp32 (queries and keys of three significant bits, 128 equal products), so the weights of equal scores are equal whatever the scores are.
+    What is left: rounding of a weight to fp16 (2^-11), fp32 sums of n weights and of the parts (2 n 2^-24 and less than 2^-20), rounding of
+    the result (2^-11, or half of the smallest step)."""
+    import torch
+    cached = [900 + 200 * i for i in range(len(q_lens))]
+    b = Batch(q_lens, cached, 40, 8, groups=groups, prefix=[700] if groups else None, width=9000 if groups else 0, seed=3)
+    r = np.random.default_rng(1)
+    b.q.zero_()
+    b.q[..., :dims] = torch.from_numpy(r.integers(4, 8, (b.rows, 40, 1)) * (size / 2)).half().cuda()
+    mark = torch.zeros(b.pages * PAGE, dtype=torch.bool, device="cuda")
+    for i, t in enumerate(b.table):
+        mark[(torch.from_numpy(t[t >= 0].astype(np.int64) * PAGE).cuda()[:, None] + torch.arange(0, PAGE, 3, device="cuda")).flatten()] = True
+    mark = mark.view(b.pages, PAGE, 1, 1)
+    live = b.k.isfinite()
+    b.k.copy_(torch.where(live, (mark & (torch.arange(HD, device="cuda") < dims)) * (1.75 * size), math.nan))
+    got = prefix(ctx, b) if groups else window(ctx, b)
+    row = 0
+    for i, (x, c) in enumerate(zip(q_lens, cached)):
+        for j in range(x):
+            pos = np.arange(c + j + 1)
+            pos = pos[(pos % PAGE) % 3 == 0]
+            page = np.where(pos < b.shared[i], b.table[b.first[i], pos // PAGE], b.table[i, pos // PAGE]).astype(np.int64)
+            v = b.v.view(-1, 8, HD)[torch.from_numpy(page * PAGE + pos % PAGE).cuda()].double()
+            want, mean = (t.mean(0).repeat_interleave(5, 0) for t in (v, v.abs()))
+            tol = want.abs() * 2.0 ** -11 + mean * (2.0 ** -11 + 4 * pos.size * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -25
+            diff = (got[row].double() - want).abs()
+            assert bool((diff <= tol).all()), (i, j, (diff / tol).nan_to_num(nan=math.inf).max().item())
+            row += 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("q_lens,groups", [([1, 1], None), ([60, 1], None), ([130], None), ([1] * 4, [0, 4]), ([1, 40], [0, 2])])
+def test_scores_that_grow_from_key_to_key(ctx, q_lens, groups, sign):
+    """Scores around +-8192 in units of the exponent (times log2 e), growing by two units per 128 keys and passing that size at another key in every row.
+    Scores are whole numbers below 2^17, exact in fp32; an exponent has up to four roundings of half a step of 8192, 2^-12 each, a weight so 2^-10, twice
+    as numerator and denominator; the rest as in `exact`."""
+    import torch
+    cached = [1400 + 60 * i for i in range(len(q_lens))]
+    b = Batch(q_lens, cached, 40, 8, groups=groups, prefix=[700] if groups else None, width=9000 if groups else 0, seed=4)
+    b.q.zero_()
+    b.q[..., 0], b.q[..., 1], b.q[..., 2] = 32.0, 1.0, 1.0
+    b.q[..., 3] = torch.arange(b.rows, device="cuda")[:, None].half()
+    for i in range(len(q_lens)):
+        pos = np.nonzero(b.seen[i])[0]
+        pos = pos[b.table[i, pos // PAGE] >= 0]
+        k = torch.zeros((pos.size, 1, HD), dtype=torch.float16, device="cuda")
+        k[..., 0], k[..., 1] = 2004.0 * sign, torch.from_numpy(pos // 8).cuda().half()[:, None]
+        k[..., 2], k[..., 3] = 18.0 if sign > 0 else -205.0, 1.0
+        b.k.view(-1, 8, HD)[b._where(i, pos)] = k
+    got = prefix(ctx, b) if groups else window(ctx, b)
+    row = 0
+    for i, (x, c) in enumerate(zip(q_lens, cached)):
+        for j in range(x):
+            pos = np.arange(c + j + 1)
+            page = np.where(pos < b.shared[i], b.table[b.first[i], pos // PAGE], b.table[i, pos // PAGE]).astype(np.int64)
+            at = torch.from_numpy(page * PAGE + pos % PAGE).cuda()
+            k, v = b.k.view(-1, 8, HD)[at].double(), b.v.view(-1, 8, HD)[at].double()
+            w = torch.softmax((k @ b.q[row, 0].double()) / math.sqrt(HD), 0)[..., None]
+            want, mean = ((w * t).sum(0).repeat_interleave(5, 0) for t in (v, v.abs()))
+            n = pos.size
+            tol = want.abs() * 2.0 ** -11 + mean * (2.0 ** -9 + 2.0 ** -11 + 4 * n * 2.0 ** -24 + 2.0 ** -20) + n * 2.0 ** -25 * v.abs().max() + 2.0 ** -25
+            diff = (got[row].double() - want).abs()
+            assert bool((diff <= tol).all()), (i, j, (diff / tol).nan_to_num(nan=math.inf).max().item())
+            row += 1
