@@ -96,6 +96,13 @@ def _num(t):
 _ROPE_APPEND = struct.Struct("@15Q3f13i64s")      # exl3_rope_append_args (include/exl3_abi.h)
 
 
+def _i32(x, name, what):
+    """a number for a C int, which would be cut to 32 bits without a word"""
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise Exl3Error(f"{what}: {name} does not fit 32 bits")
+    return x
+
+
 def _raw_stream():
     """handle of the current stream of the current device, without the objects of torch.cuda.current_stream (1.5 us)"""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -110,6 +117,14 @@ def _chk(t, dtype, name):
         raise Exl3Error(f"{name} has dtype {t.dtype}, expected {dtype}")
     if not t.is_contiguous():
         raise Exl3Error(f"{name} must be contiguous")
+
+
+def _chk_on(t, dtype, name, device):
+    """_chk for a tensor of one device: another's address would be taken for this one's"""
+    if t is None or (t.get_device() == device and t.dtype is dtype and t.is_contiguous()):
+        return
+    _chk(t, dtype, name)
+    raise Exl3Error(f"{name} must be on the context's device")
 
 
 class Ctx:
@@ -434,38 +449,44 @@ class Ctx:
                                                  kv_chunk_size, int(causal), sm_scale), "bighead_attn_paged")
 
     @staticmethod
+    def _table(block_table, what):
+        if block_table.dim() != 2:
+            raise Exl3Error(f"{what}: the block table must be [sequences, pages]")
+        return block_table.shape
+
+    @staticmethod
     def _packed(shape, cu_q, max_q_len, bsz, what):
         """(rows, row bound, heads) of a tensor [bsz,q_len,heads,128], or [rows,heads,128] with cu_q"""
         if cu_q is None:
             if len(shape) == 4 and shape[0] == bsz:
                 return bsz * shape[1], shape[1], shape[2]
         elif len(shape) == 3 and cu_q.numel() == bsz + 1:
-            return shape[0], shape[0] if max_q_len is None else max_q_len, shape[1]
+            return shape[0], shape[0] if max_q_len is None else _i32(max_q_len, "max_q_len", what), shape[1]
         raise Exl3Error(f"{what}: shape mismatch")
 
     def _rope_append(self, q, k, v, shape, pages, planes, bits, block_table, cache_seqlens, inv_freq, out_q, cu_q, max_q_len, positions, freq_axis, q_norm,
                      k_norm, norm_eps, norm_constant_bias, rope_mode, attn_factor, stream, what):
-        f16, i32 = torch.float16, torch.int32
-        _chk(k, f16, "k"); _chk(v, f16, "v"); _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens")
+        f16, i32, device = torch.float16, torch.int32, self.device
+        _chk_on(k, f16, "k", device); _chk_on(v, f16, "v", device); _chk_on(block_table, i32, "block_table", device); _chk_on(cache_seqlens, i32, "cache_seqlens", device)
         n_freq, nq, n_axes, hd = 0, 0, 1, shape[-1]
-        bsz, pps = block_table.shape
+        bsz, pps = self._table(block_table, what)
         rows, seq, nkv = self._packed(shape, cu_q, max_q_len, bsz, what)
-        good = v.shape == shape and cache_seqlens.numel() == bsz and k.get_device() == self.device
+        good = v.shape == shape and cache_seqlens.numel() == bsz
         if q is not None:
-            _chk(q, f16, "q")
+            _chk_on(q, f16, "q", device)
             full = q.shape
             nq = full[-2]
             good = good and len(full) == len(shape) and full[0] == shape[0] and full[-1] == hd and (cu_q is not None or full[1] == seq)
             if out_q is not None:
-                _chk(out_q, f16, "out_q")
+                _chk_on(out_q, f16, "out_q", device)
                 good = good and out_q.shape == full
         if inv_freq is not None:
-            _chk(inv_freq, torch.float32, "inv_freq")
+            _chk_on(inv_freq, torch.float32, "inv_freq", device)
             n_freq = inv_freq.numel()
         if cu_q is not None:
-            _chk(cu_q, i32, "cu_q")
+            _chk_on(cu_q, i32, "cu_q", device)
         if positions is not None:
-            _chk(positions, i32, "positions")
+            _chk_on(positions, i32, "positions", device)
             if positions.dim() == 2:
                 n_axes = positions.shape[0]
             good = good and positions.numel() == n_axes * rows
@@ -474,14 +495,17 @@ class Ctx:
             freq_axis = bytes(freq_axis)
         for w in (q_norm, k_norm):
             if w is not None:
-                _chk(w, f16, "q_norm / k_norm")
+                _chk_on(w, f16, "q_norm / k_norm", device)
                 good = good and w.numel() == hd
         if not good or (out_q is not None and q is None) or n_freq > 64:
-            raise Exl3Error(f"{what}: shape mismatch, or tensors that are not on the context's device")
-        args = _ROPE_APPEND.pack(_num(q), _num(out_q), k.data_ptr(), v.data_ptr(), _num(inv_freq), _num(positions), _num(q_norm), _num(k_norm),
-                                 planes[0].data_ptr(), planes[1].data_ptr(), _num(planes[2]), _num(planes[3]), block_table.data_ptr(),
-                                 cache_seqlens.data_ptr(), _num(cu_q), norm_eps, norm_constant_bias, attn_factor, n_freq, n_axes, rope_mode, bsz,
-                                 seq, rows, nq, nkv, hd, pages, pps, bits[0], bits[1], freq_axis or b"")
+            raise Exl3Error(f"{what}: shape mismatch")
+        try:
+            args = _ROPE_APPEND.pack(_num(q), _num(out_q), k.data_ptr(), v.data_ptr(), _num(inv_freq), _num(positions), _num(q_norm), _num(k_norm),
+                                     planes[0].data_ptr(), planes[1].data_ptr(), _num(planes[2]), _num(planes[3]), block_table.data_ptr(),
+                                     cache_seqlens.data_ptr(), _num(cu_q), norm_eps, norm_constant_bias, attn_factor, n_freq, n_axes, rope_mode, bsz,
+                                     seq, rows, nq, nkv, hd, pages, pps, bits[0], bits[1], freq_axis or b"")
+        except struct.error as e:                        # a number that its field does not hold
+            raise Exl3Error(f"{what}: {e}") from None
         rc = lib().exl3_rope_append_paged(self._h, self._stream(stream), args)
         if rc:
             self.check(rc, what)
@@ -491,7 +515,8 @@ class Ctx:
                           rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
         """Head norm and rotation of q and k, k and v into the fp16 pools, one launch.  positions: None, int32 [rows] or
         [axes, rows]; freq_axis: the axis of every frequency (bytes, or a list of them).  out_q None: q in place."""
-        _chk(k_cache, torch.float16, "k_cache"); _chk(v_cache, torch.float16, "v_cache")
+        device = self.device
+        _chk_on(k_cache, torch.float16, "k_cache", device); _chk_on(v_cache, torch.float16, "v_cache", device)
         cache, shape = k_cache.shape, k.shape
         if len(cache) != 4 or cache[1] != 256 or cache[2] != shape[-2] or cache[3] != shape[-1] or v_cache.shape != cache:
             raise Exl3Error("rope_append_paged: the pools must be [pages, 256, nkv, head_dim]")
@@ -502,7 +527,8 @@ class Ctx:
                             positions=None, freq_axis=None, q_norm=None, k_norm=None, norm_eps=1e-6, norm_constant_bias=0.0,
                             rope_mode=ROPE_NEOX, attn_factor=1.0, stream=None):
         """The same into the quantised pools (qk/qv int32 [pages,256,groups*bits], sk/sv fp16 [pages,256,groups])."""
-        _chk(qk, torch.int32, "qk"); _chk(qv, torch.int32, "qv"); _chk(sk, torch.float16, "sk"); _chk(sv, torch.float16, "sv")
+        device = self.device
+        _chk_on(qk, torch.int32, "qk", device); _chk_on(qv, torch.int32, "qv", device); _chk_on(sk, torch.float16, "sk", device); _chk_on(sv, torch.float16, "sv", device)
         groups = k.shape[-2] * k.shape[-1] // 32
         if (sk.shape[1:] != (256, groups) or sv.shape != sk.shape or qk.shape[:2] != sk.shape[:2] or qv.shape[:2] != sk.shape[:2] or
                 qk.shape[2] % groups or qv.shape[2] % groups or not qk.shape[2] or not qv.shape[2]):
@@ -512,15 +538,17 @@ class Ctx:
                           "rope_append_paged_q")
 
     def _span_shapes(self, q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, what):
-        f16, i32 = torch.float16, torch.int32
-        _chk(q, f16, "q"); _chk(k_cache, f16, "k_cache"); _chk(v_cache, f16, "v_cache"); _chk(o, f16, "o")
-        _chk(block_table, i32, "block_table"); _chk(cache_seqlens, i32, "cache_seqlens"); _chk(cu_q, i32, "cu_q")
-        bsz, pps = block_table.shape
+        f16, i32, device = torch.float16, torch.int32, self.device
+        _chk_on(q, f16, "q", device); _chk_on(k_cache, f16, "k_cache", device); _chk_on(v_cache, f16, "v_cache", device); _chk_on(o, f16, "o", device)
+        _chk_on(block_table, i32, "block_table", device); _chk_on(cache_seqlens, i32, "cache_seqlens", device); _chk_on(cu_q, i32, "cu_q", device)
+        bsz, pps = self._table(block_table, what)
         shape, cache = q.shape, k_cache.shape
+        if len(cache) != 4:
+            raise Exl3Error(f"{what}: the pools must be [pages, 256, nkv, head_dim]")
         rows, q_len, nq = self._packed(shape, cu_q, max_q_len, bsz, what)
         pages, page, nkv, hd = cache
-        if page != 256 or v_cache.shape != cache or o.shape != shape or shape[-1] != hd or cache_seqlens.numel() != bsz or q.get_device() != self.device:
-            raise Exl3Error(f"{what}: shape mismatch, or tensors that are not on the context's device")
+        if page != 256 or v_cache.shape != cache or o.shape != shape or shape[-1] != hd or cache_seqlens.numel() != bsz:
+            raise Exl3Error(f"{what}: shape mismatch")
         return bsz, q_len, rows, nq, nkv, hd, pages, pps
 
     def window_attn_paged(self, q, k_cache, v_cache, block_table, cache_seqlens, o, window, sinks=0, sm_scale=0.0, cu_q=None,
@@ -528,6 +556,7 @@ class Ctx:
         """Attention of q over the fp16 pools, each row seeing its last `window` tokens (itself among them) and the first
         `sinks` of its sequence; the rows' own keys are in the pools already."""
         shape = self._span_shapes(q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, "window_attn_paged")
+        window, sinks = _i32(window, "window", "window_attn_paged"), _i32(sinks, "sinks", "window_attn_paged")
         rc = lib().exl3_window_attn_paged(self._h, self._stream(stream), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                           block_table.data_ptr(), cache_seqlens.data_ptr(), _adr(cu_q), o.data_ptr(), *shape, window, sinks,
                                           sm_scale)
@@ -539,7 +568,7 @@ class Ctx:
         """Causal attention of q over the fp16 pools; sequences [group_start[g], group_start[g+1]) share their first
         prefix_lens[g] tokens, which are read once.  The rows' own keys are in the pools already."""
         shape = self._span_shapes(q, k_cache, v_cache, block_table, cache_seqlens, o, cu_q, max_q_len, "prefix_attn_paged")
-        _chk(group_start, torch.int32, "group_start"); _chk(prefix_lens, torch.int32, "prefix_lens")
+        _chk_on(group_start, torch.int32, "group_start", self.device); _chk_on(prefix_lens, torch.int32, "prefix_lens", self.device)
         n_groups = prefix_lens.numel()
         if group_start.numel() != n_groups + 1:
             raise Exl3Error("prefix_attn_paged: group_start must have one entry more than prefix_lens")

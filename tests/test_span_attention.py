@@ -584,3 +584,73 @@ def test_scores_that_grow_from_key_to_key(ctx, q_lens, groups, sign):
             diff = (got[row].double() - want).abs()
             assert bool((diff <= tol).all()), (i, j, (diff / tol).nan_to_num(nan=math.inf).max().item())
             row += 1
+
+
+class _Tensor:
+    """what the wrappers look at, without a GPU"""
+
+    def __init__(self, dtype, *shape, device=0):
+        import torch
+        self.dtype, self.shape, self.device, self.is_cuda = dtype, torch.Size(shape), device, True
+
+    def get_device(self):
+        return self.device
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def data_ptr(self):
+        return 4096
+
+
+class _Library:
+    """takes the calls of the three operators and keeps their arguments"""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append((name, a)) or 0
+
+
+@pytest.mark.parametrize("op", ["window", "prefix", "append", "append_q"])
+def test_wrappers_refuse_other_devices_and_numbers_beyond_an_int(op, monkeypatch):
+    """An address of another device would be taken for this one's, and a number of more than 32 bits would be cut: 2^32 + 5 is no window of 5."""
+    import torch
+    import exl3b200
+    from exl3b200 import ffi
+    f, i = torch.float16, torch.int32
+    rows = dict(q=(f, 2, 16, HD), block_table=(i, 2, 3), cache_seqlens=(i, 2), cu_q=(i, 3))
+    span = dict(rows, k_cache=(f, 4, PAGE, 8, HD), v_cache=(f, 4, PAGE, 8, HD), o=(f, 2, 16, HD))
+    append = dict(rows, k=(f, 2, 8, HD), v=(f, 2, 8, HD), out_q=(f, 2, 16, HD), inv_freq=(torch.float32, 64), positions=(i, 3, 2), q_norm=(f, HD), k_norm=(f, HD))
+    call, tensors, numbers = {
+        "window": ("window_attn_paged", span, dict(window=8, sinks=4)),
+        "prefix": ("prefix_attn_paged", dict(span, group_start=(i, 2), prefix_lens=(i, 1)), {}),
+        "append": ("rope_append_paged", dict(append, k_cache=(f, 4, PAGE, 8, HD), v_cache=(f, 4, PAGE, 8, HD)), dict(rope_mode=2)),
+        "append_q": ("rope_append_paged_q", dict(append, qk=(i, 4, PAGE, 128), sk=(f, 4, PAGE, 32), qv=(i, 4, PAGE, 128), sv=(f, 4, PAGE, 32)), dict(rope_mode=2)),
+    }[op]
+    numbers["max_q_len"] = 2
+    library = _Library()
+    monkeypatch.setattr(ffi, "lib", lambda: library)
+    c = exl3b200.Ctx.__new__(exl3b200.Ctx)
+    c._h, c.device = None, 0
+    good = {n: _Tensor(*t) for n, t in tensors.items()}
+    getattr(c, call)(**good, **numbers, stream=0)
+    assert len(library.calls) == 1
+    for n, t in tensors.items():
+        with pytest.raises(exl3b200.Exl3Error, match="device"):
+            getattr(c, call)(**{**good, n: _Tensor(*t, device=1)}, **numbers, stream=0)
+    for n in numbers:
+        for x in (2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1):
+            with pytest.raises(exl3b200.Exl3Error, match=call):
+                getattr(c, call)(**good, **{**numbers, n: x}, stream=0)
+    for n, t in dict(block_table=(i, 6), **({} if "append" in op else dict(k_cache=(f, 4, PAGE, 8 * HD)))).items():
+        with pytest.raises(exl3b200.Exl3Error, match=call):
+            getattr(c, call)(**{**good, n: _Tensor(*t)}, **numbers, stream=0)
+    assert len(library.calls) == 1
