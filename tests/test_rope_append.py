@@ -302,3 +302,87 @@ def test_wrapper_checks_shapes(ctx):
                    dict(q_norm=f(64)), dict(inv_freq=f(64)), dict(freq_axis=[1] * 64)):
         with pytest.raises(exl3b200.Exl3Error):
             ctx.rope_append_paged(**{**good, **change})
+
+
+# ---------------------------------------------------------------------------------------------------------------- many rows
+# From 32 rows per SM on a block takes eight rows, two of them in work.
+
+def _ragged(rows, seed):
+    """sequences of 0 to 13 rows, so that borders and empty ones fall inside a block of eight, then a long one up to `rows`"""
+    r = np.random.default_rng(seed)
+    q = [int(x) for x in r.integers(0, 14, 150)]
+    q += [rows - sum(q), 0, 3, 0]
+    q[150] -= 3
+    return q, [int(x) for x in r.integers(0, 700, len(q))]
+
+
+def _many(extra):
+    import torch
+    return 32 * torch.cuda.get_device_properties(0).multi_processor_count + extra
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [-3, 0, 1, 7])
+@pytest.mark.parametrize("heads,mode,n_freq,axes,norm,in_place", [
+    ((40, 8), 2, 64, 0, True, False), ((40, 8), 2, 48, 3, False, True), ((9, 3), 1, 33, 2, True, True), ((2, 1), 2, 64, 0, False, True), ((65, 13), 1, 64, 0, True, False),
+    ((7, 7), 0, 0, 0, True, True), ((28, 4), 2, 8, 1, False, False)])
+def test_many_rows(ctx, extra, heads, mode, n_freq, axes, norm, in_place):
+    """around the row count from which a block has eight rows; two rows behind the last sequence"""
+    q, cached = _ragged(_many(extra - 2), abs(extra + n_freq))
+    c = Case(q, cached, *heads, n_freq=n_freq, axes=axes, mode=mode, norm=norm, seed=extra + 3, extra_rows=2, cbias=0.5 if norm else 0.0, attn_factor=1.25)
+    c.table[3, :] = c.bt[3] = -1                           # and a sequence without pages
+    at = sum(q[:3])
+    c.slot[at:at + q[3]] = -1
+    c.check(ctx, in_place)
+
+
+@pytest.mark.gpu
+def test_many_rows_that_are_left_out_and_rectangular(ctx):
+    import torch
+    rows = _many(5)
+    q, cached = _ragged(rows, 5)
+    c = Case(q, cached, 12, 2, seed=9)
+    before = c.kc.clone()
+    out = c.run(ctx, max_q_len=13)                         # the long sequence has more rows than declared
+    a, b = sum(q[:150]), sum(q[:151])
+    assert bool((out[a:b] == 7.0).all()) and bool((out[:a] != 7.0).any(-1).all()) and bool((out[b:] != 7.0).any(-1).all())
+    at = torch.from_numpy(c.slot[a:b]).cuda()
+    assert torch.equal(c.kc.view(-1, 2, HD)[at], before.view(-1, 2, HD)[at])
+    n = (rows + 10) // 11
+    c = Case([11] * n, [(37 * i) % 500 for i in range(n)], 12, 2, seed=10, norm=True)
+    out = c.run(ctx)
+    kc, vc = c.kc.clone(), c.vc.clone()
+    c.kc.zero_(), c.vc.zero_()
+    got = torch.empty_like(c.q).view(n, 11, 12, HD)
+    ctx.rope_append_paged(c.q.view(n, 11, 12, HD), c.k.view(n, 11, 2, HD), c.v.view(n, 11, 2, HD), c.kc, c.vc, c.bt, c.sl, c.inv_freq, out_q=got,
+                          q_norm=c.q_norm, k_norm=c.k_norm)
+    at = torch.from_numpy(c.slot).cuda()
+    assert torch.equal(got.view(-1, 12, HD), out)
+    for x, y in ((c.kc, kc), (c.vc, vc)):
+        assert torch.equal(x.view(-1, 2, HD)[at], y.view(-1, 2, HD)[at])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (8, 3), (2, 5)])
+@pytest.mark.parametrize("nkv", [8, 3, 1])
+@pytest.mark.parametrize("extra", [0, 7])
+def test_many_rows_to_quantised_pools(ctx, extra, nkv, k_bits, v_bits):
+    import torch
+    q, cached = _ragged(_many(extra - 1), extra + nkv)
+    c = Case(q, cached, 2 * nkv, nkv, seed=k_bits, norm=True, extra_rows=1, axes=3)
+    out = c.run(ctx)
+    pools = []
+    for _ in range(2):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        codes = [torch.randint(-2 ** 31, 2 ** 31 - 1, (c.pages, PAGE, nkv * 4 * b), device="cuda", generator=g, dtype=torch.int64).int() for b in (k_bits, v_bits)]
+        scales = [torch.rand((c.pages, PAGE, nkv * 4), device="cuda", generator=g).half() for _ in range(2)]
+        pools.append((codes[0], scales[0], codes[1], scales[1]))
+    qk, sk, qv, sv = pools[0]
+    keys = torch.zeros_like(c.k)                           # its new keys as packed rows, out of the fp16 pool
+    keys[:c.rows] = c.kc.view(-1, nkv, HD)[torch.from_numpy(c.slot).cuda()]
+    ctx.quant_cache_paged(keys, qk, sk, c.v, qv, sv, c.sl, c.bt, cu_q=c.cu, seq_len=max(q))
+    got = torch.full_like(c.q, 7.0)
+    ctx.rope_append_paged_q(c.q, c.k, c.v, *pools[1], c.bt, c.sl, c.inv_freq, out_q=got, **c.kw())
+    assert torch.equal(got, out)
+    for a, b in zip(*pools):
+        assert torch.equal(a, b)
