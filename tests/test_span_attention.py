@@ -654,3 +654,65 @@ def test_wrappers_refuse_other_devices_and_numbers_beyond_an_int(op, monkeypatch
         with pytest.raises(exl3b200.Exl3Error, match=call):
             getattr(c, call)(**{**good, n: _Tensor(*t)}, **numbers, stream=0)
     assert len(library.calls) == 1
+
+
+# ------------------------------------------------------------------------------------- captured calls whose batch changes
+
+def _states(which):
+    """(most rows of a sequence, heads, window, states): batches of one call's sizes, each sequences' rows, cached tokens, groups and prefixes"""
+    r = np.random.default_rng(len(which))
+    lens = lambda n, lo, hi: [int(x) for x in r.integers(lo, hi, n)]  # noqa: E731
+    if which == "decode":                                  # prefix kernel, stream, join
+        return 1, (40, 8), BIG, [([1] * 8, lens(8, 0, 900), [0, 4, 8], [0, 0]), ([1] * 8, lens(8, 5000, 6000), [0, 8, 8], [4999, 0]),
+                                 ([1, 0] * 4, lens(8, 300, 900), [1, 2, 7], [256, 129]), ([0] * 8, lens(8, 300, 900), [0, 4, 8], [256, 129]),
+                                 ([1] * 8, lens(8, 300, 900), [0, 3, 8], [1, 300])]
+    if which == "mixed":                                   # and the sequences of many rows on tcgen05
+        return 70, (40, 8), BIG, [([1, 40, 1, 3, 9, 1], lens(6, 300, 900), [0, 3, 6], [256, 300]), ([70, 1, 0, 1, 2, 1], lens(6, 3000, 4000), [0, 6, 6], [2900, 0]),
+                                  ([1] * 6, lens(6, 0, 900), [0, 2, 4], [0, 0]), ([60, 3, 3, 3, 3, 3], lens(6, 128, 900), [2, 4, 6], [128, 100]),
+                                  ([1, 40, 1, 3, 9, 1], lens(6, 300, 900), [0, 0, 6], [9, 257])]
+    if which == "many":                                    # more sequences than a launch of the stream takes
+        return 20, (16, 8), BIG, [([1] * 1100, lens(1100, 64, 300), [0, 600, 1100], [64, 60]), ([1] * 1070 + [20] + [0] * 29, lens(1100, 200, 500), [0, 1100, 1100], [200, 0]),
+                                  ([0] * 40 + [1] * 1060, lens(1100, 0, 300), [0, 500, 1100], [0, 0]), ([20, 13] + [1] * 1060 + [0] * 38, lens(1100, 130, 300), [3, 900, 1050], [128, 1])]
+    return 251, (40, 8), 1024, [([1] * 28 + [251] * 4, lens(32, 300, 6000), None, None), ([251, 1, 1, 100] + [1] * 28, lens(32, 0, 2000), None, None),
+                                ([1] * 32, lens(32, 0, 6000), None, None), ([0] * 28 + [251, 0, 250, 4], lens(32, 2000, 6000), None, None)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["decode", "mixed", "many", "window"])
+def test_batches_that_change_between_replays(ctx, which):
+    """Wide tables, so that prefixes are read together: the prefix kernel, the kernels over own keys and the join as nodes of one graph.  Rows, lengths,
+    tables, groups and prefixes of every replay are others; each state comes twice, once behind each other one."""
+    import torch
+    import exl3b200
+    most, (nq, nkv), w, states = _states(which)
+    total = max(sum(s[0]) for s in states) + 2
+    batches = [Batch(q, c, nq, nkv, w, 4 if w != BIG else 0, groups=g, prefix=p, seed=i, extra_rows=total - sum(q), pages=2600 if which == "many" else 900,
+                     width=300) for i, (q, c, g, p) in enumerate(states)]
+    now = {n: torch.zeros_like(getattr(batches[0], n)) for n in ("q", "k", "v", "bt", "sl", "cu", "o")}
+    if w == BIG:
+        groups = [[torch.tensor(x, dtype=torch.int32, device="cuda") for x in (b.groups, b.prefix)] for b in batches]
+        start, lens = (torch.zeros_like(x) for x in groups[0])
+    graph = exl3b200.CudaGraph(ctx)
+    torch.cuda.synchronize()
+    before = ctx.launch_count()
+    graph.capture_begin()
+    args = [now[n] for n in ("q", "k", "v", "bt", "sl")]
+    kw = dict(cu_q=now["cu"], max_q_len=most, stream=graph.side_stream())
+    for _ in range(2):                                     # the second call behind the first one's join
+        if w == BIG:
+            ctx.prefix_attn_paged(*args, start, lens, now["o"], **kw)
+        else:
+            ctx.window_attn_paged(*args, now["o"], w, sinks=4, **kw)
+    graph.capture_end()
+    assert ctx.launch_count() - before == 2 * {"decode": 3, "mixed": 4, "many": 5, "window": 2}[which]
+    order = [i for a in range(len(batches)) for b in range(a) for i in (a, b)]
+    for i in order:
+        for n, t in now.items():
+            t.copy_(getattr(batches[i], n))
+        if w == BIG:
+            start.copy_(groups[i][0]), lens.copy_(groups[i][1])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        batches[i].check(now["o"])
+    ctx.poll_status()
