@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     uint64_t* meet = empty + AR_STAGES;
     int* tile_of = reinterpret_cast<int*>(smem + Cfg::OFF_TILE);                    // key tile in a stage, -1: none of its keys exist
     __shared__ int s_last;
+    __shared__ SpanLoad loads[AR_WARPS + 1];
 
     const SpanArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -107,7 +108,12 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
         const SpanTiles t = span_tiles<TK>(a, s.cached, s.cached + s.ql - 1, len);
         return max((ALONE ? (len + TK - 1) / TK : 0) + t.sink + t.near, 1);
     };
-    for (int b = tid; b < p.bsz; b += AR_THREADS) sum[b] = tiles_of(p.b0 + b);
+    SpanLoad load = {0, 0};
+    for (int b = tid; b < p.bsz; b += AR_THREADS) {
+        sum[b] = tiles_of(p.b0 + b);
+        if (a.beside) span_load(a, b, AR_ROWS, load);
+    }
+    if (a.beside) span_load_put(loads, warp, load, lane);
     __syncthreads();
     if (warp == 0) {
         int before = 0;
@@ -126,7 +132,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     // CTA's start: what fits in 32 bits is divided there.)
     auto quotient = [](long long x, int y) -> long long { return x >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y); };
     const long long F = (long long)sum[p.bsz] * n_hg;
-    const long long share = max(quotient(F + gridDim.x - 1, gridDim.x), (long long)p.min_share);
+    const int ctas = a.beside ? max(span_few_sms(a, loads, AR_WARPS + 1), 1) : gridDim.x;
+    const long long share = max(quotient(F + ctas - 1, ctas), (long long)p.min_share);
     const int c = blockIdx.x, snap = (int)min((long long)AR_SNAP, share / 4);
     auto sequence_of = [&](long long f) -> int {            // the one with tile f: sum[b] * n_hg <= f < sum[b + 1] * n_hg
         const long long per_group = quotient(f, n_hg);

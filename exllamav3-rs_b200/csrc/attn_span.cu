@@ -125,7 +125,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
         const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
                                         ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1) + 1;
-        const int grid = (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
+        const int grid = a.beside ? ctas : (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
         if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
         else exl3_launch(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
         ctx->launches++;
@@ -149,18 +149,17 @@ int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p, int sms)
     return EXL3_OK;
 }
 
-// SMs for the sequences of few rows beside those of many, from what the host knows of a batch over windows; 0: one after the other.  Long
-// sequences are at least so many as the rows need, and every one counts as full; a tile of 256 rows is 2.3 us, and an SM reads 42 GB/s.
-int span_aside(exl3_ctx* ctx, const SpanArgs& a)
+// Whether a batch over windows may have both classes, and enough of them that their kernels run beside one another, each on the SMs that
+// span_few_sms gives it: as far as the host knows, by full windows.
+bool span_beside(exl3_ctx* ctx, const SpanArgs& a)
 {
-    if (a.window > SPAN_MAX_LEN || a.q_len < 2) return 0;
+    if (a.n_groups > 0 || a.window > SPAN_MAX_LEN || a.q_len < 2 || a.bsz > AR_MAX_BSZ) return false;
     const int G = a.nq / a.nkv;
-    const double keys = std::min((double)a.window + a.sinks, (double)a.pps * EXL3_PAGE);
+    const double tiles = std::min((double)a.window + a.sinks, (double)a.pps * EXL3_PAGE) / AS_TK;
     const double n_long = std::max(0.0, std::ceil(((double)a.rows - a.bsz) / (a.q_len - 1))), n_few = a.bsz - n_long;
-    const double few = n_few * keys * a.nkv * 512 / 42e3;                                                  // us of one SM
-    const double many = n_long * std::ceil((double)a.q_len * G / 256) * a.nkv * (keys / AS_TK + 1.5) * 2.3;
-    if (n_long < 1 || n_few < 1 || few < many / 16 || many < few / 16 || few + many < 10.0 * ctx->num_sms) return 0;
-    return std::min(std::max((int)(ctx->num_sms * few / (few + many)), 8), ctx->num_sms - 8);
+    const double few = n_few * tiles * a.nkv * SPAN_FEW_TILE / 20;                                         // us of one SM
+    const double many = n_long * std::ceil((double)a.q_len * G / 256) * a.nkv * (tiles * SPAN_MANY_TILE + SPAN_MANY_UNIT) / 20;
+    return n_long >= 1 && n_few >= 1 && few >= many / 16 && many >= few / 16 && few + many >= 10.0 * ctx->num_sms;
 }
 
 int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what)
@@ -197,25 +196,29 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
         p.first = 0;
     }
     exl3_chain_scope chain(ctx, groups);
-    // Both classes of a batch over windows, where neither is small beside the other: each gets its share of the SMs, and the start and end of
-    // one kernel, 10 us and more, runs under the other (28 rows beside 4 x 251, window 1024: 89 us, one after the other 104).
-    const int aside = any_long && any_few && !groups && a.n_groups == 0 ? span_aside(ctx, a) : 0;
-    if (aside) {
+    // Both classes of a batch over windows: each gets its share of the SMs, and the start and end of one kernel, 10 us and more, runs under the
+    // other (us, and one call of each class behind the other: 28 rows beside 4 x 251, window 1024 92 and 93, 64 x 1 beside 2 x 300, window 2048 91 and 103, 28 x 1
+    // beside 251, window 4096 125 and 142; 40 x 1 at 200 tokens beside 512 at 16384 91 and 91, 120 x 1 at 20 to 300 beside 4 x 1024, window 4096 461 and 426).
+    const bool beside = any_long && any_few && span_beside(ctx, a);
+    SpanArgs both = a;
+    if (beside) {
+        both.beside = ctx->num_sms; both.unit_rows = AS_BLOCK * (two_own ? 2 : 1) / G * G;
+        p.a = both;
         if (cudaEventRecord(ctx->ev_fork, st) != cudaSuccess || cudaStreamWaitEvent(ctx->aux_stream, ctx->ev_fork, 0) != cudaSuccess)
             return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream fork failed");
         const int chained = ctx->chain;
         ctx->chain = 0;                                      // a plain launch: nothing of the second stream is in front
-        rc = a.nkv % 4 == 0 ? span_rows<4, false>(ctx, ctx->aux_stream, a, true, true, p, aside, &off)
-                            : span_rows<1, false>(ctx, ctx->aux_stream, a, true, true, p, aside, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4, false>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off)
+                            : span_rows<1, false>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off);
         ctx->chain = chained;
         ctx->chain_break = 1;
     }
     if (any_long && rc == EXL3_OK) {
         p.prefixes = 0; p.partial = own; p.share = share + 1;
-        rc = two_own ? span_tc<2>(ctx, st, p, ctx->num_sms - aside) : span_tc<1>(ctx, st, p, ctx->num_sms - aside);
+        rc = two_own ? span_tc<2>(ctx, st, p, ctx->num_sms) : span_tc<1>(ctx, st, p, ctx->num_sms);
         p.first = 0;
     }
-    if (aside) {
+    if (beside) {
         // joined after an error too, so that a capture in progress stays well-formed
         if (cudaEventRecord(ctx->ev_join, ctx->aux_stream) != cudaSuccess || cudaStreamWaitEvent(st, ctx->ev_join, 0) != cudaSuccess)
             return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream join failed");
@@ -248,7 +251,7 @@ extern "C" int exl3_window_attn_paged(exl3_ctx* ctx, exl3_stream stream, const v
                                       float sm_scale)
 {
     SpanArgs a = {(const half*)q, (half*)o, (const half*)k_cache, (const half*)v_cache, block_table, cache_seqlens, cu_q, nullptr, nullptr,
-                  bsz, q_len, rows, nq, nkv, pages, pages_per_seq, 0, window, sinks, 0.f};
+                  bsz, q_len, rows, nq, nkv, pages, pages_per_seq, 0, window, sinks, 0.f, 0, 0};
     const int rc = span_check(ctx, a, hd, sm_scale, "window_attn_paged");
     if (rc) return rc;
     EXL3_REQUIRE(window > 0 && sinks >= 0, "window_attn_paged: window must be positive and sinks not negative");
@@ -262,7 +265,7 @@ extern "C" int exl3_prefix_attn_paged(exl3_ctx* ctx, exl3_stream stream, const v
                                       int rows, int nq, int nkv, int hd, int pages, int pages_per_seq, float sm_scale)
 {
     SpanArgs a = {(const half*)q, (half*)o, (const half*)k_cache, (const half*)v_cache, block_table, cache_seqlens, cu_q, group_start, prefix_lens,
-                  bsz, q_len, rows, nq, nkv, pages, pages_per_seq, n_groups, INT_MAX, 0, 0.f};
+                  bsz, q_len, rows, nq, nkv, pages, pages_per_seq, n_groups, INT_MAX, 0, 0.f, 0, 0};
     const int rc = span_check(ctx, a, hd, sm_scale, "prefix_attn_paged");
     if (rc) return rc;
     EXL3_REQUIRE(n_groups >= 0 && n_groups <= bsz, "prefix_attn_paged: there are between 0 and bsz groups");

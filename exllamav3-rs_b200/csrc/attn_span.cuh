@@ -21,9 +21,15 @@ struct SpanArgs {
     int bsz, q_len, rows, nq, nkv, pages, pps, n_groups;
     int window, sinks;                            // window: INT_MAX without one
     float scale_log2;
+    int beside;                                   // SMs that the kernels of few and of many rows share, running beside one another; 0: each has the GPU
+    int unit_rows;                                // then: packed rows of a unit of the tcgen05 kernel
 };
 
 constexpr int SPAN_MAX_LEN = 1 << 30;
+// 1/20 us that an SM takes per kv head: for a tile of 128 keys and a few rows (64 KB at 55 GB/s), for one and 256 packed rows, and for a unit of 256 rows
+// besides; units of 128, two at a time, take 4/5.  Fitted to 12 batches at 23 splits of the SMs each: 0 to 9 % above the best of the 23, where one
+// kernel behind the other takes 4 to 44 % more.
+constexpr int SPAN_FEW_TILE = 24, SPAN_MANY_TILE = 46, SPAN_MANY_UNIT = 120;
 
 // A sequence's place in the call.  ql 0: it has no rows, more than the call declared, or rows that the call does not have.
 struct SpanSeq { int row_base, ql, cached; };
@@ -75,6 +81,42 @@ __device__ __forceinline__ SpanTiles span_tiles(const SpanArgs& a, int p_first, 
     t.sink = (min(a.sinks, t.end) + TK - 1) / TK;
     if (t.near > 0) t.sink = min(t.sink, t.first);
     return t;
+}
+
+// Where both kernels run beside one another, their split of the SMs goes by the time of an SM that either class needs, as the lengths have it: whole
+// numbers, so that every CTA of both kernels finds the same.  The load of sequence b (a tenth of a second at most):
+struct SpanLoad { unsigned few, many; };
+__device__ __forceinline__ void span_load(const SpanArgs& a, int b, int few_rows, SpanLoad& load)
+{
+    const int G = a.nq / a.nkv;
+    const SpanSeq s = span_seq(a, b);
+    if (s.ql == 0) return;
+    const int last = s.cached + s.ql - 1, packed = s.ql * G;
+    constexpr unsigned MOST = 1u << 21;                 // of 1024 sequences together 2^31
+    if (packed <= few_rows) {
+        const SpanTiles t = span_tiles<64>(a, s.cached, last, 0);
+        load.few += min((unsigned)max(t.sink + t.near, 1), MOST / SPAN_FEW_TILE) * (SPAN_FEW_TILE / 2);
+    } else {                                            // its units' tiles: halfway between the first's and the last's
+        const int step = a.unit_rows / G;
+        const SpanTiles t0 = span_tiles<128>(a, s.cached, min(s.cached + step - 1, last), 0), t1 = span_tiles<128>(a, max(last - step + 1, s.cached), last, 0);
+        const unsigned unit = min((unsigned)(t0.sink + t0.near + t1.sink + t1.near), MOST / SPAN_MANY_TILE) * (SPAN_MANY_TILE / 2) + SPAN_MANY_UNIT;
+        load.many += min((unsigned)((packed + a.unit_rows - 1) / a.unit_rows), MOST / unit) * unit;
+    }
+}
+// a warp's part of the loads, to shared memory
+__device__ __forceinline__ void span_load_put(SpanLoad* loads, int warp, const SpanLoad& load, int lane)
+{
+    const unsigned few = __reduce_add_sync(0xffffffffu, load.few), many = __reduce_add_sync(0xffffffffu, load.many);
+    if (lane == 0) loads[warp] = {few, many};
+}
+// the SMs of the kernel for few rows
+__device__ __forceinline__ int span_few_sms(const SpanArgs& a, const SpanLoad* loads, int warps)
+{
+    unsigned few = 0, many = 0;
+    for (int w = 0; w < warps; ++w) { few += loads[w].few; many += loads[w].many; }
+    if (a.unit_rows <= 128) many -= many / 5;
+    if (few == 0 || many == 0) return few ? a.beside : 0;
+    return min(max((int)__fdiv_rn(__fmul_rn((float)a.beside, (float)few), __fadd_rn((float)few, (float)many)), 4), a.beside - 4);
 }
 
 // Partial sums of a row and head: 128 dims, the exponents' reference, the sum of the weights

@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
              *kv_empty = kv_full + SLOTS, *piece_full = kv_empty + SLOTS, *piece_empty = piece_full + 2, *q_full = piece_empty + 2, *q_empty = q_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NBARS);
     __shared__ int s_failed;
+    __shared__ SpanLoad loads[SW + 2];
 
     const SpanArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     }
     // the line's length: tiles of every 32 sequences, longest unit
     int longest = 0;
+    SpanLoad load = {0, 0};
     AsEntry mine = {0, 0, 0, 0, 0, -1};                     // of the first chunk, which the producer keeps
     int tiles = 0;
     for (int ch = (warp + 2) % (SW + 2); ch < n_chunks; ch += SW + 2) {
@@ -215,7 +217,9 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == 0) sums[ch] = v;
         if (p.prefixes) longest = max(longest, (e.cached + AS_TK - 1) / AS_TK);
+        else if (a.beside && ch * 32 + lane < n) span_load(a, ch * 32 + lane, AR_ROWS, load);
     }
+    if (a.beside) span_load_put(loads, warp, load, lane);
     if (p.prefixes) {
         #pragma unroll
         for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
@@ -229,7 +233,8 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) F += __shfl_xor_sync(0xffffffffu, F, o);
     F *= a.nkv;
-    long long share = max((F + gridDim.x - 1) / gridDim.x, 1LL);
+    const int ctas = a.beside ? max(Cfg::CTAS * (a.beside - span_few_sms(a, loads, SW + 2)), 1) : gridDim.x;
+    long long share = max((F + ctas - 1) / ctas, 1LL);
     // a prefix's parts each have a place among the partial sums; with one place units stay whole, with the CTA where they begin
     const bool cut = !p.prefixes || p.max_splits > 1;
     if (p.prefixes && p.max_splits > 2) share = max(share, (long long)(sums[AS_MAX_CHUNKS] - 1) / (p.max_splits - 1) + 1);

@@ -716,3 +716,49 @@ def test_batches_that_change_between_replays(ctx, which):
         torch.cuda.synchronize()
         batches[i].check(now["o"])
     ctx.poll_status()
+
+
+# ---------------------------------------------------------------------------------------- both classes of a batch side by side
+
+LOPSIDED = [
+    # short contexts beside a chunk far into a document, the other way round, chunks at the beginning of theirs, few rows in all
+    ([1] * 40 + [256], [200] * 40 + [8000], 4096, 40, 8), ([1] * 30 + [300] * 3, [5000] * 30 + [0, 3, 9], 2048, 32, 8), ([300] * 3 + [1] * 30, [1] * 33, 4096, 40, 8),
+    ([1] * 100 + [20] * 8, [3000] * 100 + [9, 700] * 4, 2048, 40, 8), ([1] * 60 + [400, 2], [31 * i for i in range(62)], 2048, 12, 2), ([0] * 30 + [251] * 4 + [1] * 30, [999] * 64, 1024, 9, 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(LOPSIDED)))
+def test_classes_of_unlike_lengths_side_by_side(ctx, case):
+    import torch
+    q_lens, cached, w, nq, nkv = LOPSIDED[case]
+    b = Batch(q_lens, cached, nq, nkv, w, 4, seed=case, extra_rows=3, width=max(w // PAGE, 40))
+    first = window(ctx, b).clone()
+    b.check(first)
+    for _ in range(3):
+        assert torch.equal(window(ctx, b), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("few,many", [((40, 200), (1, 256, 16384)), ((120, 150), (4, 1024, 6000))])
+def test_side_by_side_is_no_detour(ctx, few, many):
+    """Decode rows with short contexts beside chunks with full windows: the classes' split of the SMs goes by lengths.  Split by the window, such calls took
+    1.5 to 2.1 times as long as the two classes in calls of their own; half as much again is the bound."""
+    import torch
+    q = [1] * few[0] + [many[1]] * many[0]
+    batches = [Batch(x, c, 40, 8, 4096, 4, seed=1) for x, c in ((q, [few[1]] * few[0] + [many[2]] * many[0]), ([1] * few[0], [few[1]] * few[0]), ([many[1]] * many[0], [many[2]] * many[0]))]
+
+    def us(b):
+        times = []
+        for _ in range(12):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for _ in range(10):
+                ctx.window_attn_paged(b.q, b.k, b.v, b.bt, b.sl, b.o, b.window, sinks=4, cu_q=b.cu, max_q_len=max(b.q_lens))
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end) * 100)
+        return sorted(times[2:])[2]
+
+    both, alone = us(batches[0]), [us(b) for b in batches[1:]]
+    assert both < 1.5 * sum(alone), (both, alone)
