@@ -72,8 +72,8 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 }
 
 // ALONE: prefixes are read here too, through their own table, by each sequence.  (A kernel of its own: with both kinds of tiles in every loop
-// 128 rows over windows of 4096 took 210 us for 193, a row over 1024 13.4 for 12.6.)
-template <int HW, bool ALONE>
+// 128 rows over windows of 4096 took 210 us for 193, a row over 1024 13.4 for 12.6.)  BESIDE: the other kernel runs at the same time.
+template <int HW, bool ALONE, bool BESIDE>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_constant__ ArMaps maps, const ArParams p, int early)
 {
     using Cfg = ArCfg<HW>;
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     uint64_t* meet = empty + AR_STAGES;
     int* tile_of = reinterpret_cast<int*>(smem + Cfg::OFF_TILE);                    // key tile in a stage, -1: none of its keys exist
     __shared__ int s_last;
-    __shared__ SpanLoad loads[AR_WARPS + 1];
+    __shared__ SpanLoad loads[BESIDE ? AR_WARPS + 1 : 1];
 
     const SpanArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -111,9 +111,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     SpanLoad load = {0, 0};
     for (int b = tid; b < p.bsz; b += AR_THREADS) {
         sum[b] = tiles_of(p.b0 + b);
-        if (a.beside) span_load(a, b, AR_ROWS, load);
+        if (BESIDE) span_load(a, b, AR_ROWS, load);
     }
-    if (a.beside) span_load_put(loads, warp, load, lane);
+    if (BESIDE) span_load_put(loads, warp, load, lane);
     __syncthreads();
     if (warp == 0) {
         int before = 0;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const __grid_c
     // CTA's start: what fits in 32 bits is divided there.)
     auto quotient = [](long long x, int y) -> long long { return x >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y); };
     const long long F = (long long)sum[p.bsz] * n_hg;
-    const int ctas = a.beside ? max(span_few_sms(a, loads, AR_WARPS + 1), 1) : gridDim.x;
+    const int ctas = BESIDE ? max(span_few_sms(a, loads, AR_WARPS + 1), 1) : gridDim.x;
     const long long share = max(quotient(F + ctas - 1, ctas), (long long)p.min_share);
     const int c = blockIdx.x, snap = (int)min((long long)AR_SNAP, share / 4);
     auto sequence_of = [&](long long f) -> int {            // the one with tile f: sum[b] * n_hg <= f < sum[b + 1] * n_hg

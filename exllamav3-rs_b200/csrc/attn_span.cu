@@ -100,7 +100,7 @@ constexpr size_t AR_SCRATCH = (size_t)AR_WARPS * AR_ROWS * AR_MS * 4;       // p
 // Keys that a CTA takes at least: fewer are more partial sums to join (us at 64, 128 and 192 keys: one row over a window of 1024 16.2, 15.5 and
 // 20.7, of 4096 26, 20 and 23)
 constexpr int AR_MIN_KEYS = 128;
-template <int HW, bool ALONE>
+template <int HW, bool ALONE, bool BESIDE = false>
 int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, bool plain, const AsParams& pre, int sms, size_t* ws_off)
 {
     using Cfg = ArCfg<HW>;
@@ -110,7 +110,7 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     if (Cfg::KW == 1) { maps.k16 = maps.k; maps.v16 = maps.v; }
     static bool done[64] = {};
-    if (!span_configure(attn_rows_kernel<HW, ALONE>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    if (!span_configure(attn_rows_kernel<HW, ALONE, BESIDE>, Cfg::BYTES, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int ctas = sms;
     ArParams p;
     p.a = a;
@@ -125,26 +125,26 @@ int span_rows(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, bool first, boo
         // no more CTAs than there can be shares: a sequence has at most the tiles of its window and first keys, or of its table
         const long long most = std::min((long long)a.pps * (EXL3_PAGE / Cfg::TK),
                                         ((long long)std::min(a.window, SPAN_MAX_LEN) + AR_ROWS) / Cfg::TK + 2 + std::min(a.sinks, SPAN_MAX_LEN) / Cfg::TK + 1) + 1;
-        const int grid = a.beside ? ctas : (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
-        if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
-        else exl3_launch(ctx, attn_rows_kernel<HW, ALONE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
+        const int grid = BESIDE ? ctas : (int)std::min((long long)ctas, std::max(1LL, (most * p.bsz * (a.nkv / HW) + p.min_share - 1) / p.min_share));
+        if (p.first && !plain) exl3_launch_first(ctx, attn_rows_kernel<HW, ALONE, BESIDE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p);
+        else exl3_launch(ctx, attn_rows_kernel<HW, ALONE, BESIDE>, grid, AR_THREADS, Cfg::BYTES, st, maps, p, 0);
         ctx->launches++;
     }
     return EXL3_OK;
 }
 
 // a launch of the tcgen05 kernel with NB row blocks per CTA
-template <int NB>
+template <int NB, bool BESIDE = false>
 int span_tc(exl3_ctx* ctx, cudaStream_t st, const AsParams& p, int sms)
 {
     CUtensorMap kmap, vmap, qmap;
     if (!span_map(p.a, p.a.kc, AS_TK, 2, 1, &kmap) || !span_map(p.a, p.a.vc, AS_TK, 2, 1, &vmap) || !span_q_map(p.a, AsCfg<NB>::ROWS, &qmap))
         return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: no tensor map of the pools");
     static bool done[64] = {};
-    if (!span_configure(attn_span_kernel<NB>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
+    if (!span_configure(attn_span_kernel<NB, BESIDE>, AsCfg<NB>::SMEM, ctx->device, done)) return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: shared memory");
     const int grid = AsCfg<NB>::CTAS * sms;
-    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p);
-    else exl3_launch(ctx, attn_span_kernel<NB>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p, 0);
+    if (p.first) exl3_launch_first(ctx, attn_span_kernel<NB, BESIDE>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p);
+    else exl3_launch(ctx, attn_span_kernel<NB, BESIDE>, grid, AsCfg<NB>::THREADS, AsCfg<NB>::SMEM, st, kmap, vmap, qmap, p, 0);
     ctx->launches++;
     return EXL3_OK;
 }
@@ -208,14 +208,15 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
             return exl3_fail(ctx, EXL3_ERR_CUDA, "attention: stream fork failed");
         const int chained = ctx->chain;
         ctx->chain = 0;                                      // a plain launch: nothing of the second stream is in front
-        rc = a.nkv % 4 == 0 ? span_rows<4, false>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off)
-                            : span_rows<1, false>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off);
+        rc = a.nkv % 4 == 0 ? span_rows<4, false, true>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off)
+                            : span_rows<1, false, true>(ctx, ctx->aux_stream, both, true, true, p, ctx->num_sms, &off);
         ctx->chain = chained;
         ctx->chain_break = 1;
     }
     if (any_long && rc == EXL3_OK) {
         p.prefixes = 0; p.partial = own; p.share = share + 1;
-        rc = two_own ? span_tc<2>(ctx, st, p, ctx->num_sms) : span_tc<1>(ctx, st, p, ctx->num_sms);
+        rc = beside ? two_own ? span_tc<2, true>(ctx, st, p, ctx->num_sms) : span_tc<1, true>(ctx, st, p, ctx->num_sms)
+                    : two_own ? span_tc<2>(ctx, st, p, ctx->num_sms) : span_tc<1>(ctx, st, p, ctx->num_sms);
         p.first = 0;
     }
     if (beside) {

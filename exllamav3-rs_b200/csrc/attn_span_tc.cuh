@@ -170,7 +170,8 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b)
     return o;
 }
 
-template <int NB>
+// BESIDE: the kernel of few rows runs at the same time (a kernel of its own: the code for it cost calls without it 1 to 2 us)
+template <int NB, bool BESIDE>
 __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                                          const __grid_constant__ CUtensorMap vmap,
                                                                                          const __grid_constant__ CUtensorMap qmap,
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
              *kv_empty = kv_full + SLOTS, *piece_full = kv_empty + SLOTS, *piece_empty = piece_full + 2, *q_full = piece_empty + 2, *q_empty = q_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::NBARS);
     __shared__ int s_failed;
-    __shared__ SpanLoad loads[SW + 2];
+    __shared__ SpanLoad loads[BESIDE ? SW + 2 : 1];
 
     const SpanArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -217,9 +218,9 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == 0) sums[ch] = v;
         if (p.prefixes) longest = max(longest, (e.cached + AS_TK - 1) / AS_TK);
-        else if (a.beside && ch * 32 + lane < n) span_load(a, ch * 32 + lane, AR_ROWS, load);
+        else if (BESIDE && ch * 32 + lane < n) span_load(a, ch * 32 + lane, AR_ROWS, load);
     }
-    if (a.beside) span_load_put(loads, warp, load, lane);
+    if (BESIDE) span_load_put(loads, warp, load, lane);
     if (p.prefixes) {
         #pragma unroll
         for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(AsCfg<NB>::THREADS, AsCfg<NB>::CTAS) attn_span
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) F += __shfl_xor_sync(0xffffffffu, F, o);
     F *= a.nkv;
-    const int ctas = a.beside ? max(Cfg::CTAS * (a.beside - span_few_sms(a, loads, SW + 2)), 1) : gridDim.x;
+    const int ctas = BESIDE ? max(Cfg::CTAS * (a.beside - span_few_sms(a, loads, SW + 2)), 1) : gridDim.x;
     long long share = max((F + ctas - 1) / ctas, 1LL);
     // a prefix's parts each have a place among the partial sums; with one place units stay whole, with the CTA where they begin
     const bool cut = !p.prefixes || p.max_splits > 1;
