@@ -8,7 +8,8 @@
 //
 // A tile is 32 KB of keys and values, for four warps: HW = 4 heads side by side and 16 keys, a head per warp, where the kv heads come in
 // fours - 1 KB of every token in one piece, and no warp needs another - else one head and 64 keys, 16 per warp, which meet at the end of
-// a unit.  (One head and 64 keys of 8: 128 rows over windows of 4096, 256-byte pieces, 262 us; as it is 191 us, 6.2 TB/s.)
+// a unit.  (One head and 64 keys of 8: 128 rows over windows of 4096, 256-byte pieces, 262 us, where as it is it took 191; 193 to 210 us on the
+// machines it was timed on since, 5.6 to 6.1 TB/s.)
 //
 // A sequence and head group whose tiles fall to several CTAs goes through partial sums, which the one that arrives last adds up in the
 // order of the tiles: results do not depend on who that is.  Keys of a tile that no row sees are not loaded where they fill a group of 16,

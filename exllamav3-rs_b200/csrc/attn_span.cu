@@ -168,9 +168,10 @@ int span_run(exl3_ctx* ctx, cudaStream_t st, const SpanArgs& a, const char* what
     const int G = a.nq / a.nkv;
     const long long packed = (long long)a.q_len * G, all = (long long)a.rows * G;
     const bool any_long = packed > AR_ROWS, any_few = G <= AR_ROWS && (a.cu_q || !any_long);
-    // A few sequences of few rows read a short prefix sooner each than together, which is two kernels more: up to 128 MB read again (as far as the
-    // host knows, from the table's width).  us, each and together, 16 / 8 heads, sequences x prefix: 4 x 512 18 and 30, 8 x 2048 24 and 32,
-    // 16 x 2048 36 and 39, 32 x 1024 37 and 34; 40 / 8 heads: 4 x 8192 41 and 44, 8 x 8192 59 and 46.
+    // A few sequences of few rows read a short prefix sooner each than together, which is two kernels more: up to 128 MB read again, as far as the
+    // host knows, which is the table's width: tables much wider than the prefix take the way together.  us, each and together, 16 / 8 heads,
+    // sequences x prefix: 4 x 512 17 and 27, 8 x 2048 24 and 31, 16 x 2048 35 and 38, 32 x 1024 37 and 29; 40 / 8 heads: 4 x 8192 42 and 39,
+    // 8 x 8192 57 and 41.
     const bool alone = a.n_groups > 0 && !any_long && (double)(a.bsz - 1) * a.pps * EXL3_PAGE * a.nkv * 512 <= 128.0 * (1 << 20);
     const bool groups = a.n_groups > 0 && !alone;
     // Two row blocks share the tiles where a group or a sequence may have that many rows

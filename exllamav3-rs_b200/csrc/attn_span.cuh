@@ -27,8 +27,8 @@ struct SpanArgs {
 
 constexpr int SPAN_MAX_LEN = 1 << 30;
 // 1/20 us that an SM takes per kv head: for a tile of 128 keys and a few rows (64 KB at 55 GB/s), for one and 256 packed rows, and for a unit of 256 rows
-// besides; units of 128, two at a time, take 4/5.  Fitted to 12 batches at 23 splits of the SMs each: 0 to 9 % above the best of the 23, where one
-// kernel behind the other takes 4 to 44 % more.
+// besides; units of 128, two at a time, take 4/5.  Fitted to 12 batches at 23 splits of the SMs each: 0 to 9 % above the best of the 23, where the
+// classes in calls of their own take 3 to 44 % more than that.
 constexpr int SPAN_FEW_TILE = 24, SPAN_MANY_TILE = 46, SPAN_MANY_UNIT = 120;
 
 // A sequence's place in the call.  ql 0: it has no rows, more than the call declared, or rows that the call does not have.

@@ -10,15 +10,16 @@
 // chain of scores, softmax, product that a block cannot overlap with itself.  So an SM holds two blocks, whose softmax runs under the
 // other's products: NB = 2, one CTA whose blocks share every tile, where sequences have the rows (with two CTAs that read tiles of their own
 // 4 x 2048 rows took 794 us: 64 KB per 2500 cycles and SM is what L2 gives); NB = 1, two CTAs of one block, where they do not, so that
-// the start and end of short units overlap.  4 x 2048 rows over windows of 4096: 712 us, 845 TFLOP/s; 8 x 128 rows over 8192 shared keys and 512 to
-// 2000 of their own: 846 us, 815 TFLOP/s.  (A quarter or a sixth of the exponentials by a polynomial instead: 728 and 720 for 725 us, so
-// they are not what a tile waits for; P announced after 96 keys instead of 64: 710 and 893 for 712 and 846 us.)
+// the start and end of short units overlap.  4 x 2048 rows over windows of 4096, 40 / 8 heads: 736 to 750 us, 800 to 820 TFLOP/s; 8 x 128 rows over
+// 32768 shared keys and up to 300 of their own, 690 GFLOP, with the join: 872 to 882 us, 780 to 790 TFLOP/s.  (Tried on an earlier build: a
+// quarter or a sixth of the exponentials by a polynomial 728 and 720 us for 725, so they are not what a tile waits for; P announced after 96
+// keys instead of 64 710 for 712 and, over shared keys, 893 for 846.)
 //
 // Queries come as copies of whole rows, a unit ahead: a unit has rows * G <= 128 NB packed rows (read by the softmax threads at a unit's
 // start instead: 4 x 2048 rows 779 us).
 //
 // The tiles of all units stand in one line, of which every CTA takes an equal part (one item per CTA, with the splits chosen for the fewest
-// waves, left SMs idle for 30 % of 8 x 128 rows over 8192 shared keys: 160 units on 148 SMs).  The parts are found from the lengths by each
+// waves, left SMs idle for 30 % of 8 x 128 rows over a shared prefix: 160 units on 148 SMs).  The parts are found from the lengths by each
 // CTA itself, which costs about two microseconds once and saves a launch in front.  A unit cut by the border of a part goes through
 // partial sums: of a prefix they stay for span_join_kernel, which adds them to each sequence's own; of a sequence's own span the warp that
 // arrives last with its 32 rows adds them up in the order of the parts.

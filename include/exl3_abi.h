@@ -233,6 +233,8 @@ EXL3_API int exl3_rope_append_paged(exl3_ctx* ctx, exl3_stream stream, const exl
  * exl3_paged_kv_cache_update).  Block-table entries none of whose keys is visible are not read, so pages behind the window can be
  * released (and their entries be -1); the keys of an entry outside the pool are left out.  A row that sees nothing gives zeros.  sm_scale
  * 0 = 1/sqrt(hd), negative ones are refused.
+ * Scores, maxima, sums and partial results are held in 32 bits; a weight (relative to its row's maximum, or to one at most 2^8 below it) is rounded to fp16
+ * where it enters the product with the values, and the output once.  Scaled scores may be as large as 32 bits hold.
  * What no row of a sequence sees may hold anything; a value that is not finite at a key that some of a sequence's (or group's) rows see can
  * reach those that do not.  o must not overlap q or the pools.  Limits, EXL3_ERR_UNSUPPORTED beyond: 128 query heads per kv head, 8192
  * sequences, 2^31 key tiles by the rows' and tables' sizes; rows * nq <= 2^30.  Partial sums go to the context's scratch: 10 MB for
@@ -247,7 +249,10 @@ EXL3_API int exl3_window_attn_paged(exl3_ctx* ctx, exl3_stream stream, const voi
  * as exl3_pool_alloc_prefix gives them, or copies - and are read once for the whole group, through the block table of its first sequence.
  * The keys behind them, and all keys of sequences in no group, are read through a sequence's own table.  A sequence that has cached less
  * than the prefix is computed on its own.  A group's first table has to hold the prefix also where that sequence has no rows, or has cached
- * less.  Otherwise as above; scratch: rows * nq * 528 bytes twice over at least (and up to a quarter of the scratch, for prefixes split among
+ * less.  Where every sequence has at most 16 rows as above and (bsz - 1) * pages_per_seq * nkv is at most 1024, each sequence reads its group's prefix
+ * itself, in one kernel instead of three: a table no wider than the sequences need is faster for a few short prefixes (four sequences over 512
+ * tokens 17 us, in a table of 512 pages 24 to 27).
+ * Otherwise as above; scratch: rows * nq * 528 bytes twice over at least (and up to a quarter of the scratch, for prefixes split among
  * more SMs) beside the window's. */
 EXL3_API int exl3_prefix_attn_paged(exl3_ctx* ctx, exl3_stream stream, const void* q, const void* k_cache, const void* v_cache,
                            const int32_t* block_table, const int32_t* cache_seqlens, const int32_t* cu_q, const int32_t* group_start,
